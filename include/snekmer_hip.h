@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define SKM_ABI_VERSION 7
+#define SKM_ABI_VERSION 8
 
 #define SKM_OK 0
 #define SKM_E_BADARG (-1)
@@ -74,6 +74,13 @@ int skm_create(int device_id, skm_ctx **out_ctx);
  * against 10.5 ms per step unconfined and 10.8 on one stream; no reference counterpart: one process per FASTA file,
  * snekmer/rules/kmerize.smk:57-65).  SKM_E_UNSUPPORTED on devices with fewer than 64 or more than 512 CUs. */
 int skm_create_confined(int device_id, int first_cu_group, int last_cu_group, skm_ctx **out_ctx);
+/* A context over the caller's own stream (a hipStream_t of `device_id`; NULL: the null stream), e.g. the current stream of
+ * another library whose arrays the calls read and write: what both queue there runs in order, with no wait between.  The
+ * stream stays the caller's and has to outlive the context.  While its owner captures it, only calls without scratch
+ * memory can be made (SKM_E_UNSUPPORTED otherwise): a graph captured with skm_graph_begin knows when it is stale.
+ * skm_pointer_device: the device whose memory d_ptr points into, -1 for anything else.  No reference counterparts. */
+int skm_create_on_stream(int device_id, void *stream, skm_ctx **out_ctx);
+int skm_pointer_device(const void *d_ptr, int *h_device);
 int skm_destroy(skm_ctx *ctx);
 /* Ordering between two contexts of one process on one device (a context is one stream): skm_event_record marks the
  * current end of ctx's stream in slot [0, SKM_EVENT_SLOTS); skm_stream_wait makes everything queued on ctx from now
@@ -374,6 +381,58 @@ int skm_pairwise_f64(skm_ctx *ctx, int metric, double p, int64_t n, int64_t m, i
  * second slot holds index 0xFFFFFFFF and value 0. */
 int skm_row_top2(skm_ctx *ctx, int64_t n, int64_t m, const float *d_scores, int64_t ld, uint32_t *d_idx,
                  float *d_val);
+
+/* Log probabilities of given labels under rows of class scores, with the entropy and the k best alternatives: what a
+ * materialised score block (skm_cosine_csr against family totals, skm_linear) says beyond skm_row_top2.  No reference
+ * counterpart in this form (rules/apply.smk:312-328 looks the difference of the two best scores up in a table).
+ *   d_scores [rows x cols], row stride ld >= cols elements of any alignment; dtype 0 float32, 1 float16, 2 bfloat16
+ *   d_mask   NULL, or bytes: 0 where a class may not be chosen; row stride ldmask >= cols, 0: one row for all
+ *   d_labels the given class of each row (label_bits 32 or 64, signed), -1: none
+ *   p = softmax(scores / temperature) over the allowed classes: mask != 0 and score > -infinity
+ * Outputs (float32 / int32; each may be NULL):
+ *   d_logp[rows]        log p(label); 0 for label -1; -infinity where the label is not allowed
+ *   d_entropy[rows]     in nats
+ *   d_stats[2 * rows]   the largest allowed score m and l = log(sum of exp((score - m) / temperature)):
+ *                       log p(j) = (score_j - m) / temperature - l; what the backward pass needs
+ *   d_top_index, d_top_logp [rows x k], 0 <= k <= 16: the best classes, larger scores first, lower indices first among
+ *                       equal scores; -1 and -infinity behind the last allowed class
+ * A row without an allowed class: stats -infinity, logp -infinity, entropy 0.  A row that allows a NaN or +infinity has
+ * no distribution: NaN everywhere, indices -1.  A label outside [-1, cols) gives NaN, and the next skm_sync reports it.
+ * Differences of scores are taken before the temperature divides, the sums are float32, and S + 1 is never formed where
+ * one class holds nearly all of the mass (log1p).  Few long rows take scratch memory. */
+int skm_log_probabilities(skm_ctx *ctx, int dtype, int64_t rows, int64_t cols, const void *d_scores, int64_t ld,
+                          const uint8_t *d_mask, int64_t ldmask, const void *d_labels, int label_bits, int k,
+                          double temperature, float *d_logp, float *d_entropy, float *d_stats, int32_t *d_top_index,
+                          float *d_top_logp);
+
+/* Gradient of sum(grad_logp * logp + grad_entropy * entropy) with respect to the scores, in their type: 0 where a class
+ * is not allowed.  d_grad_logp or d_grad_entropy may be NULL (0); a row with label -1 takes nothing from grad_logp, and one
+ * whose label is not allowed what (j == label) - p leaves at the others: -p.  d_stats
+ * (and d_entropy, with d_grad_entropy) are the forward pass's.  d_grad_scores, row stride ldg, may be d_scores itself
+ * (with ldg == ld); any other overlap is refused. */
+int skm_log_probabilities_backward(skm_ctx *ctx, int dtype, int64_t rows, int64_t cols, const void *d_scores, int64_t ld,
+                                   const uint8_t *d_mask, int64_t ldmask, const void *d_labels, int label_bits,
+                                   double temperature, const float *d_stats, const float *d_entropy,
+                                   const float *d_grad_logp, const float *d_grad_entropy, void *d_grad_scores, int64_t ldg);
+
+/* y = act(x w^T + bias) + residual on the matrix cores: x [m x k], w [n x k], bias [n] or NULL, residual [m x n] or NULL,
+ * all of one type (dtype 0 float32, 1 float16, 2 bfloat16), row strides in elements, any alignment; float32 sums, each output
+ * rounded once.  activation 0 none, 1 relu, 2 gelu (erf), 3 gelu (tanh), 4 silu, 5 sigmoid.  d_preact [m x n] or NULL
+ * receives z = x w^T + bias for the backward pass.  y may be the residual itself; any other overlap of an output with an
+ * input is refused.  k = 0 is an empty sum.  Rows that do not start on 16-byte boundaries are copied to scratch first, and
+ * small outputs with a long contraction are summed in parts held in scratch.  No reference counterpart in this form: the
+ * reference hands its feature matrices to scikit-learn's estimators (snekmer/model.py). */
+int skm_linear(skm_ctx *ctx, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void *d_x, int64_t ldx,
+               const void *d_w, int64_t ldw, const void *d_bias, const void *d_residual, int64_t ldr, void *d_preact,
+               int64_t ldp, void *d_y, int64_t ldy);
+
+/* dz = dy act'(preact): dx = dz w, dw = dz^T x, dbias = column sums of dz, each in the operands' type; NULL: not wanted
+ * (then w, or x, may be NULL too).  The residual's gradient is dy.  dz is rounded to that type once for the two products
+ * (dbias sums the unrounded values).  d_preact is only read where activation is not 0.  No output may share memory with an
+ * input or another output. */
+int skm_linear_backward(skm_ctx *ctx, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void *d_dy,
+                        int64_t lddy, const void *d_preact, int64_t ldp, const void *d_x, int64_t ldx, const void *d_w,
+                        int64_t ldw, void *d_dx, int64_t lddx, void *d_dw, int64_t lddw, void *d_dbias);
 
 /* Learn aggregation (snekmer/rules/learn.smk:385-408): sum the count rows of each group
  * (annotation).  Input CSR rows carry a group id < ngroups (d_group[n]); output is the CSR of the

@@ -18,7 +18,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SNEKMER_HIP_LIB") or os.path.join(_HERE, "libsnekmer_hip.so")
 
 SKM_OK = 0
-ABI_VERSION = 7  # SKM_ABI_VERSION of include/snekmer_hip.h
+ABI_VERSION = 8  # SKM_ABI_VERSION of include/snekmer_hip.h
 ERRORS = {-1: "BADARG", -2: "NOMEM", -3: "HIP", -4: "OVERFLOW", -5: "UNSUPPORTED", -6: "COMM", -7: "STALE"}
 COMM_ID_BYTES = 128
 EVENT_SLOTS = 8  # SKM_EVENT_SLOTS
@@ -61,6 +61,8 @@ _SIGNATURES = {
     "skm_get_option": (C.c_int, [C.c_char_p, C.c_char_p, C.c_int]),
     "skm_create": (C.c_int, [C.c_int, C.POINTER(_p)]),
     "skm_create_confined": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(_p)]),
+    "skm_create_on_stream": (C.c_int, [C.c_int, _p, C.POINTER(_p)]),
+    "skm_pointer_device": (C.c_int, [_p, C.POINTER(C.c_int)]),
     "skm_destroy": (C.c_int, [_p]),
     "skm_sync": (C.c_int, [_p]),
     "skm_graph_begin": (C.c_int, [_p]),
@@ -140,6 +142,16 @@ _SIGNATURES = {
     "skm_cosine_dense_f64": (C.c_int, [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, C.c_int, _p, _i64]),
     "skm_matrix_row_stats": (C.c_int, [_p, _i64, _i64, _p, _i64, _p, _p]),
     "skm_apply_top2": (C.c_int, [_p, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p, _p, _p]),
+    "skm_log_probabilities": (C.c_int, [_p, C.c_int, _i64, _i64, _p, _i64, _p, _i64, _p, C.c_int, C.c_int, C.c_double, _p, _p, _p, _p, _p]),
+    "skm_log_probabilities_backward": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _p, _i64, _p, _i64, _p, C.c_int, C.c_double, _p, _p, _p, _p, _p, _i64],
+    ),
+    "skm_linear": (C.c_int, [_p, C.c_int, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _i64]),
+    "skm_linear_backward": (
+        C.c_int,
+        [_p, C.c_int, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p],
+    ),
     "skm_fasta_index": (C.c_int, [_p, _i64, C.c_int, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(C.c_int)]),
     "skm_fasta_parse": (C.c_int, [_p, _i64, C.c_int, _i64, _i64, _p, _p, _p, _p]),
     "skm_csr_to_dense_i8": (C.c_int, [_p, _i64, _p, _p, _p, _i64, _p, _p, _p]),
@@ -269,8 +281,29 @@ def device_count() -> int:
     return n.value
 
 
+# 16-bit brain floats, which numpy has no type for: the two raw bytes that other libraries' array interfaces name "V2"
+bfloat16 = np.dtype("V2")
+
+
+def to_bfloat16(values) -> np.ndarray:
+    """float32 values -> bfloat16 words (dtype `bfloat16`), rounded to nearest, ties to even; NaN stays NaN."""
+    f = np.ascontiguousarray(values, dtype=np.float32)
+    bits = f.view(np.uint32)
+    out = ((bits + (((bits >> np.uint32(16)) & np.uint32(1)) + np.uint32(0x7FFF))) >> np.uint32(16)).astype(np.uint16)
+    out = np.where(np.isnan(f), ((bits >> np.uint32(16)) | np.uint32(0x40)).astype(np.uint16), out)
+    return np.ascontiguousarray(out, dtype=np.uint16).view(bfloat16)
+
+
+def from_bfloat16(words) -> np.ndarray:
+    """bfloat16 words (as DeviceArray.download gives them) -> float32 values, exactly."""
+    return (np.ascontiguousarray(words).view(np.uint16).astype(np.uint32) << np.uint32(16)).view(np.float32)
+
+
 class DeviceArray:
-    """A typed 1-D/2-D view of device memory owned by a Context."""
+    """A typed 1-D/2-D view of device memory owned by a Context.  Other libraries read it in place through
+    `__cuda_array_interface__` (torch.as_tensor(array, device="cuda"), cupy.asarray(array)); they have to order their own
+    streams behind the context's (Context.sync, or a context over their stream: Context(stream=...)).  bfloat16 has no
+    name there that every reader knows: pass such a library's own array as the output instead."""
 
     def __init__(self, ctx: "Context", shape, dtype):
         self.ctx = ctx
@@ -298,6 +331,13 @@ class DeviceArray:
         except Exception:
             pass
 
+    @property
+    def __cuda_array_interface__(self) -> dict:
+        if self.ptr is None:
+            raise ValueError("the array has been freed")
+        typestr = "<V2" if self.dtype == bfloat16 else self.dtype.str
+        return {"shape": self.shape, "typestr": typestr, "data": (self.ptr, False), "strides": None, "version": 2}
+
     def upload(self, host: np.ndarray) -> "DeviceArray":
         host = np.ascontiguousarray(host, dtype=self.dtype)
         if host.size != self.size:
@@ -321,21 +361,89 @@ class DeviceArray:
         return self.ptr + int(offset_elems) * self.dtype.itemsize
 
 
+FLOAT_TYPES = {"<f4": 0, "<f2": 1, "<V2": 2}  # dtype codes of skm_linear and skm_log_probabilities
+_FLOAT_DTYPES = (np.dtype(np.float32), np.dtype(np.float16), bfloat16)
+_ITEMSIZE = {"<f4": 4, "<f2": 2, "<V2": 2, "|u1": 1, "|b1": 1, "|i1": 1, "<i4": 4, "<i8": 8}
+
+
+def float_dtype(code: int) -> np.dtype:
+    return _FLOAT_DTYPES[code]
+
+
+def is_device_array(x) -> bool:
+    return isinstance(x, DeviceArray) or hasattr(type(x), "__cuda_array_interface__")
+
+
+def array_view(ctx: "Context", x, name: str, ndim: int, types, writable: bool = False):
+    """(pointer, shape, row stride in elements, type string) of a device array of this library or of another one
+    (`__cuda_array_interface__`), as the entry points take them: the elements of a row next to each other, rows that do not
+    overlap, on the context's device, of one of `types`.  Anything else raises TypeError / ValueError naming `name`."""
+    if isinstance(x, DeviceArray):
+        if x.ptr is None:
+            raise ValueError(f"{name}: the array has been freed")
+        device, shape, ptr, typestr, strides = x.ctx.device, x.shape, x.ptr, x.dtype.str, None
+        if typestr == "|V2":
+            typestr = "<V2"
+    else:
+        iface = getattr(x, "__cuda_array_interface__", None)
+        if iface is None:
+            raise TypeError(f"{name}: want an array on the device (a DeviceArray or an object with __cuda_array_interface__), got {type(x).__name__}")
+        shape, typestr, (ptr, readonly), strides = iface["shape"], iface["typestr"], iface["data"], iface.get("strides")
+        if iface.get("mask") is not None:
+            raise ValueError(f"{name}: masked arrays are not taken")
+        if writable and readonly:
+            raise ValueError(f"{name}: the array is read-only")
+        where = getattr(x, "device", None)
+        device = getattr(where, "index", None)
+        if not isinstance(device, int):
+            device = getattr(where, "id", None)
+        if not isinstance(device, int):
+            device = ctx.device
+            if ptr:
+                out = C.c_int(-1)
+                _check(ctx.lib, ctx.lib.skm_pointer_device(_p(ptr), C.byref(out)))
+                device = out.value
+    if typestr not in types:
+        raise TypeError(f"{name}: elements of type {typestr}, want one of {', '.join(types)}")
+    if device != ctx.device:
+        raise ValueError(f"{name}: the array is on device {device}, the context on {ctx.device}")
+    if len(shape) != ndim:
+        raise ValueError(f"{name}: {len(shape)} dimensions, want {ndim}")
+    cols = shape[-1]
+    ld = cols
+    if strides is not None:
+        size = _ITEMSIZE[typestr]
+        if cols > 1 and strides[-1] != size:
+            raise ValueError(f"{name}: the elements of a row must lie next to each other")
+        if ndim == 2 and shape[0] > 1:
+            ld, rest = divmod(strides[0], size)
+            if rest or ld < cols:
+                raise ValueError(f"{name}: rows that overlap, run backwards or start between elements")
+    return ptr, shape, ld, typestr
+
+
 class Context:
     """One device + one HIP stream (skm_ctx).  Not re-entrant: one host thread at a time per context (the
     small-batch arena of engine.recode_host / kmer_codes_host is per context and unguarded); distinct contexts may be
     used from distinct threads."""
 
-    def __init__(self, device: int = 0, cu_groups: Optional[Tuple[int, int]] = None):
+    def __init__(self, device: int = 0, cu_groups: Optional[Tuple[int, int]] = None, stream: Optional[int] = None):
         """`cu_groups=(first, last)`: the context's stream may only use those compute-unit groups of 0..7
-        (skm_create_confined): a side context for work that should run beside another context's kernels."""
+        (skm_create_confined): a side context for work that should run beside another context's kernels.
+        `stream`: the handle of a stream of the caller's (0: the null stream) that the context works on instead of one of
+        its own (skm_create_on_stream), e.g. ``torch.cuda.current_stream().cuda_stream``: calls are ordered with whatever
+        its owner queues there.  The stream has to outlive the context."""
+        if stream is not None and cu_groups is not None:
+            raise ValueError("a context over the caller's stream cannot be confined to compute-unit groups")
         self.lib = load_library()
         if device_count() <= device:
             raise HipUnavailable(
                 f"no HIP device {device} visible ({device_count()} found); snekmer_amd has no CPU fallback"
             )
         handle = _p()
-        if cu_groups is None:
+        if stream is not None:
+            _check(self.lib, self.lib.skm_create_on_stream(device, _p(int(stream)), C.byref(handle)))
+        elif cu_groups is None:
             _check(self.lib, self.lib.skm_create(device, C.byref(handle)))
         else:
             _check(self.lib, self.lib.skm_create_confined(device, int(cu_groups[0]), int(cu_groups[1]), C.byref(handle)))

@@ -1,5 +1,5 @@
 """apply: the counts -> family totals -> cosine -> top-2 chain of ``snekmer learn`` / ``snekmer apply``
-on the device.
+on the device, and the log probabilities of annotations under such scores.
 
 Reference code replaced (all per sequence / per basis k-mer in Python + pandas):
   per-annotation sums of count rows      snekmer/rules/learn.smk:385-408
@@ -13,7 +13,7 @@ from typing import Optional, Sequence, Tuple
 
 import numpy as np
 
-from . import engine
+from . import _hip, engine
 
 _p = C.c_void_p
 _i64 = C.c_int64
@@ -137,6 +137,130 @@ def apply_top2(ctx, csr: engine.CountsCSR, ncols: int, totals: engine.CountsCSR,
             dot.download(2 * rows).reshape(rows, 2))
 
 
+class LogProbabilities:
+    """What `log_probabilities` computes, as device arrays (float32; top_index int32), one row per score row: `logp` [n] of the
+    given labels, `entropy` [n] in nats, `stats` [n, 2] (largest allowed score m, l with log p(j) = (score_j - m) / T - l; the
+    backward pass reads them), `top_index` / `top_logp` [n, k] of the best classes.  Members that are None are not computed."""
+
+    __slots__ = ("logp", "entropy", "stats", "top_index", "top_logp")
+
+    def __init__(self, logp=None, entropy=None, stats=None, top_index=None, top_logp=None):
+        self.logp, self.entropy, self.stats, self.top_index, self.top_logp = logp, entropy, stats, top_index, top_logp
+
+    def host(self) -> dict:
+        """The members that are DeviceArrays, as numpy arrays by name."""
+        got = {name: getattr(self, name) for name in self.__slots__}
+        return {name: a.download() for name, a in got.items() if isinstance(a, _hip.DeviceArray)}
+
+
+_LABEL_TYPES = {"<i4": 32, "<i8": 64}
+MAX_ALTERNATIVES = 16
+
+
+def _score_arguments(ctx, scores, labels, mask, ncols, temperature):
+    """The arguments that both passes share, checked: (dtype code, rows, cols, scores, ld, mask, ldmask, labels, label_bits)
+    and what has to live until the call has been queued."""
+    sp, (rows, cols), ld, t = _hip.array_view(ctx, scores, "scores", 2, _hip.FLOAT_TYPES)
+    if ncols is not None:
+        if not 0 < int(ncols) <= cols:
+            raise ValueError(f"ncols: {ncols} of {cols} columns")
+        cols = int(ncols)
+    if cols < 1:
+        raise ValueError("scores: no classes")
+    if not 0.0 < float(temperature) < float("inf"):
+        raise ValueError(f"temperature: {temperature} (want a positive number)")
+    mp, ldmask = None, 0
+    if mask is not None:
+        two = len(mask.shape) == 2
+        mp, ms, ldmask, _ = _hip.array_view(ctx, mask, "mask", 2 if two else 1, ("|u1", "|b1"))
+        engine._expect("mask", ms, (rows, cols) if two else (cols,))
+        ldmask = ldmask if two else 0
+    lp, bits, keep = None, 32, None
+    if labels is not None:
+        if not _hip.is_device_array(labels):
+            host = np.asarray(labels)
+            if host.dtype.kind not in "iu" and host.size:
+                raise TypeError(f"labels: {host.dtype} (want integers)")
+            if host.size and (host.min() < -1 or host.max() >= cols):
+                raise ValueError(f"labels: outside -1 .. {cols - 1}")
+            labels = keep = ctx.to_device(host.astype(np.int32).reshape(host.shape))
+        lp, ls, _, lt = _hip.array_view(ctx, labels, "labels", 1, _LABEL_TYPES)
+        engine._expect("labels", ls, (rows,))
+        bits = _LABEL_TYPES[lt]
+    return (_hip.FLOAT_TYPES[t], rows, cols, sp, ld, mp, ldmask, lp, bits), keep
+
+
+def _packed(ctx, x, name, shape, types, writable=False):
+    """Pointer of an array of this shape whose elements all lie next to each other, None for None."""
+    if x is None:
+        return None
+    ptr, got, ld, _ = _hip.array_view(ctx, x, name, len(shape), types, writable=writable)
+    engine._expect(name, got, shape)
+    if len(shape) == 2 and ld != shape[1]:
+        raise ValueError(f"{name}: rows must lie next to each other")
+    return ptr
+
+
+def log_probabilities(ctx, scores, labels=None, k: int = 0, temperature: float = 1.0, mask=None, ncols: Optional[int] = None,
+                      out: Optional[LogProbabilities] = None) -> LogProbabilities:
+    """softmax(scores / temperature) by rows, of a score block resident on the device (skm_log_probabilities): the log
+    probability of each row's given label, the entropy, and the k best classes, ties towards the lower column as in
+    `row_top2`.  What `learn_apply(materialize=True)` / `cosine_rows_vs_totals` / `engine.linear` produce, read as a
+    distribution over annotations: where the reference maps the difference of the two best scores to a confidence
+    (snekmer/rules/apply.smk:320-326), this says how likely each annotation is under the scores.
+
+    `scores` [n, ld] float32, float16 or `_hip.bfloat16`, of which the first `ncols` columns count (default: all); `labels` [n]:
+    class ids on the device (int32 / int64) or on the host, -1 where none is known (log probability 0); `mask`: uint8 or bool
+    on the device, 0 where a class may not be chosen, [ncols] for all rows or [n, ncols]; a score of -infinity is a class that
+    may not be chosen either.  `k` <= 16 alternatives, padded with (-1, -inf).  A row that allows nothing has entropy 0 and
+    log probability -inf; one that allows a NaN or +inf is NaN throughout, with indices -1.  A label on the device outside
+    [-1, ncols) gives NaN and is reported by the next Context.sync / download.  `out`: a LogProbabilities whose members are
+    filled (arrays of this library or of another one); only those it has are computed."""
+    args, keep = _score_arguments(ctx, scores, labels, mask, ncols, temperature)
+    rows = args[1]
+    k = int(k)
+    if not 0 <= k <= MAX_ALTERNATIVES:
+        raise ValueError(f"k: {k} alternatives (0 to {MAX_ALTERNATIVES})")
+    if out is None:
+        out = LogProbabilities(ctx.empty(rows, np.float32) if labels is not None else None, ctx.empty(rows, np.float32), ctx.empty((rows, 2), np.float32),
+                               ctx.empty((rows, k), np.int32) if k else None, ctx.empty((rows, k), np.float32) if k else None)
+    if out.logp is not None and labels is None:
+        raise ValueError("labels: log probabilities need them")
+    if not k and (out.top_index is not None or out.top_logp is not None):
+        raise ValueError("k: the alternatives' arrays are given, but k is 0")
+    f32 = ("<f4",)
+    ctx.call("skm_log_probabilities", *args, k, float(temperature), _packed(ctx, out.logp, "logp", (rows,), f32, True),
+             _packed(ctx, out.entropy, "entropy", (rows,), f32, True), _packed(ctx, out.stats, "stats", (rows, 2), f32, True),
+             _packed(ctx, out.top_index, "top_index", (rows, k), ("<i4",), True), _packed(ctx, out.top_logp, "top_logp", (rows, k), f32, True))
+    return out
+
+
+def log_probabilities_backward(ctx, scores, labels, forward: LogProbabilities, d_logp=None, d_entropy=None, temperature: float = 1.0, mask=None,
+                               ncols: Optional[int] = None, out=None):
+    """Gradient of ``(d_logp * logp + d_entropy * entropy).sum()`` with respect to the scores, in their type
+    (skm_log_probabilities_backward).  `forward`: what `log_probabilities` left for the same scores, labels, mask and
+    temperature (`stats`, and `entropy` if `d_entropy` is given).  Classes that may not be chosen get 0; columns of `out`
+    behind `ncols` are left as they are.  `out` may be `scores` itself.  Alternatives carry no gradient."""
+    args, keep = _score_arguments(ctx, scores, labels, mask, ncols, temperature)
+    code, rows, cols = args[:3]
+    if d_logp is None and d_entropy is None:
+        raise ValueError("d_logp, d_entropy: one of them is needed")
+    if d_logp is not None and labels is None:
+        raise ValueError("labels: the gradient of the log probabilities needs them")
+    if forward.stats is None or (d_entropy is not None and forward.entropy is None):
+        raise ValueError("forward: stats (and entropy, for d_entropy) are needed")
+    f32 = ("<f4",)
+    if out is None:
+        out = ctx.empty((rows, cols), _hip.float_dtype(code))
+    gp, gs, ldg, _ = _hip.array_view(ctx, out, "out", 2, tuple(t for t, c in _hip.FLOAT_TYPES.items() if c == code), writable=True)
+    if gs[0] != rows or gs[1] < cols or (ncols is None and gs[1] != cols):
+        raise ValueError(f"out: shape {tuple(gs)}, want {(rows, cols)}")
+    ctx.call("skm_log_probabilities_backward", *args, float(temperature), _packed(ctx, forward.stats, "stats", (rows, 2), f32),
+             _packed(ctx, forward.entropy, "entropy", (rows,), f32), _packed(ctx, d_logp, "d_logp", (rows,), f32),
+             _packed(ctx, d_entropy, "d_entropy", (rows,), f32), gp, ldg)
+    return out
+
+
 def confidence_lookup(delta: np.ndarray, table) -> np.ndarray:
     """``vals["delta"].map(global_confidence_scores)`` of rules/apply.smk:325-326: the confidence of
     every (already rounded) delta from the global confidence table, NaN where the table has no such
@@ -164,11 +288,16 @@ def predict(ctx, csr: engine.CountsCSR, ncols: int, totals: engine.CountsCSR, la
     return out
 
 
-def learn_apply(ctx, csr: engine.CountsCSR, ncols: int, groups: Sequence[int], ngroups: int, materialize: bool = False, basis=None):
+def learn_apply(ctx, csr: engine.CountsCSR, ncols: int, groups: Sequence[int], ngroups: int, materialize: bool = False, basis=None,
+                alternatives: Optional[int] = None, temperature: float = 1.0):
     """Self-evaluation chain of rules/learn.smk: totals per annotation, cosine of every sequence
     against every annotation, top-2 and delta (rounded to 2 decimals as learn.smk:842/apply.smk:325).
     The N x A score block is only produced when `materialize` is set (the save_apply_associations
-    branch of apply.smk:298-301 writes it out)."""
+    branch of apply.smk:298-301 writes it out).  With `alternatives` (0 to 16; needs the block) the block is also read as a
+    distribution over the annotations: out["log_probabilities"] is `log_probabilities` of every sequence's own annotation
+    with that many best alternatives at `temperature`."""
+    if alternatives is not None and not materialize:
+        raise ValueError("alternatives: only read from the materialised block (materialize=True)")
     totals = group_sum(ctx, csr, groups, ngroups, basis=basis, ncols=ncols)
     # rows of one annotation next to each other: they share their family's k-mers (see apply_top2)
     idx, score, dot = apply_top2(ctx, csr, ncols, totals, order=np.argsort(np.asarray(groups), kind="stable"))
@@ -176,4 +305,6 @@ def learn_apply(ctx, csr: engine.CountsCSR, ncols: int, groups: Sequence[int], n
            "delta": np.round(score[:, 0] - score[:, 1], 2)}
     if materialize:
         out["scores"], out["ld"] = cosine_rows_vs_totals(ctx, csr, ncols, totals)
+        if alternatives is not None:
+            out["log_probabilities"] = log_probabilities(ctx, out["scores"], groups, k=alternatives, temperature=temperature, ncols=ngroups)
     return out

@@ -139,7 +139,8 @@ namespace {
 // first_group < 0: an ordinary stream.  Otherwise the context's stream is confined to the CU groups first..last of 0..7
 // (mask bit i: group (i / 8) % 8 - every group has eight CUs in every XCD -, as the two streams of the overlapped cosine
 // schedule are).
-int create_ctx(int device_id, int first_group, int last_group, skm_ctx **out_ctx, const char *who)
+// foreign: the stream is the caller's.
+int create_ctx(int device_id, int first_group, int last_group, skm_ctx **out_ctx, const char *who, bool foreign = false, hipStream_t theirs = nullptr)
 {
     SKM_REQUIRE(out_ctx, SKM_E_BADARG, "%s: null output", who);
     *out_ctx = nullptr;
@@ -151,7 +152,14 @@ int create_ctx(int device_id, int first_group, int last_group, skm_ctx **out_ctx
     SKM_HIP(hipGetDeviceProperties(&prop, device_id));
     hipStream_t stream = nullptr;
     int usable = prop.multiProcessorCount;
-    if (first_group >= 0) {
+    if (foreign) {
+        stream = theirs;
+        if (stream) {  // (a stream belongs to one device for good)
+            hipDevice_t dev = -1;
+            SKM_HIP(hipStreamGetDevice(stream, &dev));
+            SKM_REQUIRE((int)dev == device_id, SKM_E_BADARG, "%s: the stream belongs to device %d, not %d", who, (int)dev, device_id);
+        }
+    } else if (first_group >= 0) {
         const int ncu = prop.multiProcessorCount;
         SKM_REQUIRE(first_group <= last_group && last_group <= 7, SKM_E_BADARG, "%s: CU groups %d..%d (want 0 <= first <= last <= 7)", who,
                     first_group, last_group);
@@ -180,13 +188,15 @@ int create_ctx(int device_id, int first_group, int last_group, skm_ctx **out_ctx
     ctx->num_cus = prop.multiProcessorCount;
     ctx->usable_cus = usable;
     ctx->stream = stream;
+    ctx->foreign = foreign;
     ctx->cu_first = first_group;
     ctx->cu_last = last_group;
     {
         const hipError_t e = skm_pinned_acquire(device_id, &ctx->h_pinned);  // zeroed (offset 2048: the previous cosine call's heavy-row count)
         if (e != hipSuccess) {
             (void)hipGetLastError();
-            skm_stream_release(device_id, first_group, last_group, stream);
+            if (!foreign)
+                skm_stream_release(device_id, first_group, last_group, stream);
             delete ctx;
             skm_set_error("%s: pinned page: %s", who, hipGetErrorString(e));
             return SKM_E_NOMEM;
@@ -210,6 +220,25 @@ extern "C" int skm_create_confined(int device_id, int first_cu_group, int last_c
     SKM_REQUIRE(first_cu_group >= 0, SKM_E_BADARG, "skm_create_confined: CU groups %d..%d (want 0 <= first <= last <= 7)", first_cu_group,
                 last_cu_group);
     return create_ctx(device_id, first_cu_group, last_cu_group, out_ctx, "skm_create_confined");
+}
+
+extern "C" int skm_create_on_stream(int device_id, void *stream, skm_ctx **out_ctx)
+{
+    return create_ctx(device_id, -1, -1, out_ctx, "skm_create_on_stream", true, (hipStream_t)stream);
+}
+
+extern "C" int skm_pointer_device(const void *d_ptr, int *h_device)
+{
+    SKM_REQUIRE(h_device, SKM_E_BADARG, "skm_pointer_device: null output");
+    *h_device = -1;
+    hipPointerAttribute_t at;
+    if (!d_ptr || hipPointerGetAttributes(&at, d_ptr) != hipSuccess) {  // not an address that the runtime knows
+        (void)hipGetLastError();
+        return SKM_OK;
+    }
+    if (at.type == hipMemoryTypeDevice || at.type == hipMemoryTypeManaged)
+        *h_device = at.device;
+    return SKM_OK;
 }
 
 extern "C" int skm_destroy(skm_ctx *ctx)
@@ -250,7 +279,8 @@ extern "C" int skm_destroy(skm_ctx *ctx)
         skm_event_release(ctx->device, false, e);
     skm_stream_release(ctx->device, -1, -1, ctx->s_writer);
     skm_stream_release(ctx->device, 0, 3, ctx->s_gram);
-    skm_stream_release(ctx->device, ctx->cu_first, ctx->cu_last, ctx->stream);
+    if (!ctx->foreign)
+        skm_stream_release(ctx->device, ctx->cu_first, ctx->cu_last, ctx->stream);
     delete ctx;
     return SKM_OK;
 }
@@ -309,6 +339,11 @@ int skm_check_device_error(skm_ctx *ctx, const char *who)
     if (bits & SKM_DEVERR_SEQ_TOO_LONG) {
         skm_set_error("%s: an earlier skm_count_csr / skm_vectorize_csr call on this context was given a max_seq_len smaller than "
                       "one of its sequences; the rows of those sequences were left EMPTY (pass 0 or a true bound)", who);
+        return SKM_E_BADARG;
+    }
+    if (bits & SKM_DEVERR_LABEL) {
+        skm_set_error("%s: an earlier skm_log_probabilities / skm_log_probabilities_backward call on this context was given a label outside "
+                      "[-1, cols); those rows' log probabilities and gradients were set to NaN", who);
         return SKM_E_BADARG;
     }
     skm_set_error("%s: a kernel reported error bits 0x%x", who, bits);
@@ -444,6 +479,9 @@ int skm_ws(skm_ctx *ctx, int slot, size_t bytes, void **out)
 {
     if (bytes < 256)
         bytes = 256;
+    // a graph that somebody else captures would keep this address without the check of skm_graph_launch
+    SKM_REQUIRE(!skm_foreign_capture(ctx), SKM_E_UNSUPPORTED,
+                "a call that needs scratch while the owner of the context's stream captures it: capture with skm_graph_begin instead");
     if (ctx->ws_bytes[slot] < bytes) {
         if (ctx->capturing) {
             skm_set_error("scratch slot %d would grow (%zu -> %zu bytes) inside skm_graph_begin .. skm_graph_end: run the same calls "
@@ -497,6 +535,8 @@ extern "C" int skm_graph_begin(skm_ctx *ctx)
 {
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     SKM_REQUIRE(!ctx->capturing, SKM_E_BADARG, "skm_graph_begin: a capture is already open on this context");
+    SKM_REQUIRE(!ctx->foreign || ctx->stream, SKM_E_UNSUPPORTED, "skm_graph_begin: the null stream cannot be captured; use a context on another stream");
+    SKM_REQUIRE(!skm_foreign_capture(ctx), SKM_E_BADARG, "skm_graph_begin: the owner of the context's stream is capturing it");
     SKM_HIP(hipSetDevice(ctx->device));
     // relaxed mode: other threads (and this one) may allocate and free while the capture is open; what is captured is
     // exactly what the library queues on this context's stream

@@ -42,6 +42,7 @@ struct skm_ctx {
     hipStream_t stream = nullptr;
     int num_cus = 0;
     int usable_cus = 0;  // compute units the context's stream may use (num_cus unless skm_create_confined masked some out)
+    bool foreign = false;  // `stream` is the caller's (skm_create_on_stream; nullptr: the null stream): never destroyed or recycled here
     int cu_first = -1, cu_last = -1;  // the CU groups of a confined context's stream (-1: unmasked): the key of the stream cache
     void *ws[WS_COUNT] = {};
     size_t ws_bytes[WS_COUNT] = {};
@@ -93,9 +94,12 @@ hipEvent_t skm_event_acquire(int device, bool timing);
 void skm_event_release(int device, bool timing, hipEvent_t e);
 hipError_t skm_pinned_acquire(int device, void **out_page4096);
 void skm_pinned_release(int device, void *page);
+// true while the owner of a foreign stream captures it (not through skm_graph_begin): nothing there may be queried or waited for
+bool skm_foreign_capture(const skm_ctx *ctx);
 void skm_graph_release(struct skm_graph *graph);
 constexpr int SKM_DEVERR_WORD = 768;  // byte 3072 of h_pinned
 constexpr uint32_t SKM_DEVERR_SEQ_TOO_LONG = 1u;
+constexpr uint32_t SKM_DEVERR_LABEL = 2u;
 // Call after a stream synchronise: reports (once) what kernels flagged since the last check.
 int skm_check_device_error(skm_ctx *ctx, const char *who);
 // similarity -> distance in place over a float32 block: out = clamp(1 - out, 0, 2), no diagonal rule (the epilogue of
@@ -131,6 +135,21 @@ struct skm_lut256 {
 };
 
 static inline int64_t skm_ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Whether the cells of [ra x ca] at a (row stride lda) and [rb x cb] at b can share memory.  Column blocks of one matrix
+// interleave without sharing any.
+static inline bool skm_overlap(const void *a, int64_t ra, int64_t ca, int64_t lda, const void *b, int64_t rb, int64_t cb, int64_t ldb, int64_t es)
+{
+    if (!a || !b || ra <= 0 || rb <= 0 || ca <= 0 || cb <= 0)
+        return false;
+    const int64_t pa = (int64_t)(uintptr_t)a, pb = (int64_t)(uintptr_t)b;
+    if (pa + ((ra - 1) * lda + ca) * es <= pb || pb + ((rb - 1) * ldb + cb) * es <= pa)
+        return false;
+    if (lda != ldb || (pb - pa) % es)
+        return true;
+    const int64_t d = (((pb - pa) / es) % lda + lda) % lda;  // where b's first column lies in a's rows
+    return !(d >= ca && d + cb <= lda);
+}
 
 // Grid cap for grid-stride kernels: enough workgroups to fill 256 CUs several times over.
 static inline int skm_grid_cap(const skm_ctx *ctx, int64_t want, int per_cu = 8)

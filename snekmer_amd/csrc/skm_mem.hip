@@ -129,7 +129,7 @@ hipEvent_t take_event(device_pool *p, int timing)
 template <typename F>
 void for_streams(const skm_ctx *c, F &&f)
 {
-    if (c->stream)
+    if (c->stream || c->foreign)  // (a foreign stream may be the null stream)
         f(c->stream);
     if (c->s_writer)
         f(c->s_writer);
@@ -140,7 +140,7 @@ void for_streams(const skm_ctx *c, F &&f)
 bool any_capture(const device_pool *p)
 {
     for (const skm_ctx *c : p->contexts)
-        if (c->capturing)
+        if (c->capturing || skm_foreign_capture(c))
             return true;
     return false;
 }
@@ -198,7 +198,7 @@ bool block_idle(device_pool *p, parked_block &b)
 void quiesce_locked(device_pool *p)
 {
     for (const skm_ctx *c : p->contexts) {
-        if (c->capturing)
+        if (c->capturing || skm_foreign_capture(c))
             continue;
         for_streams(c, [&](hipStream_t s) {
             if (hipStreamSynchronize(s) != hipSuccess)
@@ -272,6 +272,18 @@ void shutdown_at_exit()
 }
 
 }  // namespace
+
+bool skm_foreign_capture(const skm_ctx *ctx)
+{
+    if (!ctx->foreign || ctx->capturing)
+        return false;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(ctx->stream, &st) != hipSuccess) {  // the null stream while another stream is being captured
+        (void)hipGetLastError();
+        return true;
+    }
+    return st != hipStreamCaptureStatusNone;
+}
 
 // ---------------------------------------------------------------------------- registry
 void skm_registry_add(skm_ctx *ctx)
@@ -393,6 +405,8 @@ void skm_pinned_release(int device, void *page)
 int skm_pool_alloc(skm_ctx *ctx, size_t bytes, void **out)
 {
     *out = nullptr;
+    SKM_REQUIRE(!skm_foreign_capture(ctx), SKM_E_UNSUPPORTED,
+                "an allocation while the owner of the context's stream captures it: allocate before, or capture with skm_graph_begin");
     device_pool *p = pool_of(ctx->device);
     if (!p) {  // the process is exiting (or an impossible device number)
         SKM_HIP(hipMalloc(out, bytes ? bytes : 1));

@@ -586,6 +586,103 @@ def cosine_dense_i8(ctx, n: int, m: int, kdim: int, x_i8, y_i8, x_rnorm, y_rnorm
     return out
 
 
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
+
+
+def _activation(name) -> int:
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation: {name!r} is not one of {', '.join(sorted(a for a in ACTIVATIONS if a))}") from None
+
+
+def _expect(name: str, shape, want) -> None:
+    if tuple(shape) != tuple(want):
+        raise ValueError(f"{name}: shape {tuple(shape)}, want {tuple(want)}")
+
+
+def linear(ctx, x, w, bias=None, activation=None, residual=None, preact=None, out=None):
+    """``act(x @ w.T + bias) + residual`` on the matrix cores (skm_linear): x [m, k], w [n, k], bias [n], residual [m, n], all
+    float32, float16 or `_hip.bfloat16`, arrays of this library or of another one (`_hip.array_view`; rows may be strided),
+    summed in float32.  `activation`: one of `ACTIVATIONS`.  `preact`: an array [m, n] that receives ``x @ w.T + bias``, or
+    True for a new one (the call then returns (y, preact)): what `linear_backward` needs for an activation.  `out` [m, n]: a new
+    array unless given; it may be `residual` itself.  For feature rows under learned weights, where `cosine_dense_i8` compares
+    count rows with each other."""
+    xp, xs, ldx, t = _hip.array_view(ctx, x, "x", 2, _hip.FLOAT_TYPES)
+    types = (t,)
+    wp, ws, ldw, _ = _hip.array_view(ctx, w, "w", 2, types)
+    (m, k), n = xs, ws[0]
+    _expect("w", ws, (n, k))
+    bp = rp = zp = None
+    ldr = ldz = n
+    if bias is not None:
+        bp, bs, _, _ = _hip.array_view(ctx, bias, "bias", 1, types)
+        _expect("bias", bs, (n,))
+    if residual is not None:
+        rp, rs, ldr, _ = _hip.array_view(ctx, residual, "residual", 2, types)
+        _expect("residual", rs, (m, n))
+    code = _hip.FLOAT_TYPES[t]
+    both = preact is True
+    if both:
+        preact = ctx.empty((m, n), _hip.float_dtype(code))
+    if preact is not None:
+        zp, zs, ldz, _ = _hip.array_view(ctx, preact, "preact", 2, types, writable=True)
+        _expect("preact", zs, (m, n))
+    if out is None:
+        out = ctx.empty((m, n), _hip.float_dtype(code))
+    yp, ys, ldy, _ = _hip.array_view(ctx, out, "out", 2, types, writable=True)
+    _expect("out", ys, (m, n))
+    ctx.call("skm_linear", code, _activation(activation), m, n, k, xp, ldx, wp, ldw, bp, rp, ldr, zp, ldz, yp, ldy)
+    return (out, preact) if both else out
+
+
+def linear_backward(ctx, dy, x, w, activation=None, preact=None, dx=True, dw=True, dbias=True):
+    """The gradients of `linear` (skm_linear_backward): with ``dz = dy * act'(preact)``, ``dx = dz @ w``, ``dw = dz.T @ x`` and
+    ``dbias = dz.sum(0)``; the residual's gradient is `dy` itself.  `dx`, `dw`, `dbias`: True for a new array, an array to fill,
+    or None / False where it is not wanted (`w` is only needed for dx, `x` only for dw; pass None).  Returns (dx, dw, dbias)."""
+    gp, gs, ldg, t = _hip.array_view(ctx, dy, "dy", 2, _hip.FLOAT_TYPES)
+    types, code = (t,), _hip.FLOAT_TYPES[t]
+    m, n = gs
+    act = _activation(activation)
+    zp = xp = wp = None
+    ldz = n
+    if act:
+        if preact is None:
+            raise ValueError(f"preact: the slope of {activation} needs the pre-activation values")
+        zp, zs, ldz, _ = _hip.array_view(ctx, preact, "preact", 2, types)
+        _expect("preact", zs, (m, n))
+    k = None
+    ldx = ldw = 0
+    if dx is not None and dx is not False and w is None:
+        raise ValueError("w: dx needs it")
+    if dw is not None and dw is not False and x is None:
+        raise ValueError("x: dw needs it")
+    if x is not None:
+        xp, xs, ldx, _ = _hip.array_view(ctx, x, "x", 2, types)
+        k = xs[1]
+        _expect("x", xs, (m, k))
+    if w is not None:
+        wp, ws, ldw, _ = _hip.array_view(ctx, w, "w", 2, types)
+        k = ws[1] if k is None else k
+        _expect("w", ws, (n, k))
+
+    def result(given, name, shape):
+        if given is None or given is False:
+            return None, None, shape[-1]
+        if given is True:
+            given = ctx.empty(shape, _hip.float_dtype(code))
+        ptr, got, ld, _ = _hip.array_view(ctx, given, name, len(shape), types, writable=True)
+        _expect(name, got, shape)
+        return given, ptr, ld
+
+    k = 0 if k is None else k
+    dx, dxp, lddx = result(dx, "dx", (m, k))
+    dw, dwp, lddw = result(dw, "dw", (n, k))
+    dbias, dbp, _ = result(dbias, "dbias", (n,))
+    ctx.call("skm_linear_backward", code, act, m, n, k, gp, ldg, zp, ldz, xp, ldx, wp, ldw, dxp, lddx, dwp, lddw, dbp)
+    return dx, dw, dbias
+
+
 class NeighborLists:
     """Exact sparse Gram rows of a row block: per row the rows j sharing a k-mer and the int32 dot."""
 
