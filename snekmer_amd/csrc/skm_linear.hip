@@ -34,28 +34,25 @@ struct ln_type<0> {
     using T = float;
     using V = f32x4;  // 16 bytes of an operand row
     static constexpr int VE = 4;
-    // the two lane halves hold columns 0-3 and 4-7 of a 32-byte step: the i-th product takes columns i and 4 + i of both
-    static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c)
-    {
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[0], b[0], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[1], b[1], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[2], b[2], c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_32x32x2f32(a[3], b[3], c, 0, 0, 0);
-    }
+    // the two lane halves hold columns 0-3 and 4-7 of a 32-byte step: part i takes columns i and 4 + i of both
+    static constexpr int PARTS = 4;
+    static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c, int i) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0); }
 };
 template <>
 struct ln_type<1> {
     using T = _Float16;
     using V = f16x8;
     static constexpr int VE = 8;
-    static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static constexpr int PARTS = 1;
+    static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c, int) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct ln_type<2> {
     using T = __bf16;
     using V = bf16x8;
     static constexpr int VE = 8;
-    static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static constexpr int PARTS = 1;
+    static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c, int) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
 // ---- activations (float32)
@@ -124,122 +121,292 @@ struct ln_gemm {
     float *partial;             // split contraction: [nsplit][m][n] float32, rows of ldq (n rounded up to 4)
     int64_t ldq;
     int nsplit;
-    int64_t stages_per_split;
+    int64_t stages, stages_per_split;  // of the contraction, LN_BK bytes each
 };
 
 __device__ const uint4 ln_zero_block = {0, 0, 0, 0};  // what lanes past the end of the contraction fetch
 
-// bias, activation and residual of VE consecutive cells of one row, and the stores
+// 16 bytes of a row, `whole` if all of them are columns of the matrix
 template <int DT, int VE>
-__device__ __forceinline__ void ln_finish(const ln_gemm &g, int64_t i, int64_t j, float (&v)[VE])
+__device__ __forceinline__ void ln_read(const typename ln_type<DT>::T *from, bool whole, int64_t left, typename ln_type<DT>::T (&v)[VE])
+{
+    static_assert(VE * sizeof(v[0]) == 16, "16 bytes");
+    if (whole) {
+        const ln_u128 raw = *reinterpret_cast<const ln_u128 *>(from);
+        __builtin_memcpy(v, &raw, 16);
+    } else {
+#pragma unroll
+        for (int u = 0; u < VE; ++u)
+            v[u] = u < left ? from[u] : (typename ln_type<DT>::T)0.0f;
+    }
+}
+template <int DT, int VE>
+__device__ __forceinline__ void ln_write(typename ln_type<DT>::T *to, bool whole, int64_t left, const float (&v)[VE])
+{
+    typename ln_type<DT>::T o[VE];
+#pragma unroll
+    for (int u = 0; u < VE; ++u)
+        o[u] = (typename ln_type<DT>::T)v[u];
+    if (whole) {
+        ln_u128 raw;
+        __builtin_memcpy(&raw, o, 16);
+        *reinterpret_cast<ln_u128 *>(to) = raw;
+    } else {
+#pragma unroll
+        for (int u = 0; u < VE; ++u)
+            if (u < left)
+                to[u] = o[u];
+    }
+}
+
+// bias, activation and residual of VE consecutive cells (i, j ..) and the stores; `left` = columns from j on
+template <int DT, int VE>
+__device__ __forceinline__ void ln_cells(const ln_gemm &g, int act, int64_t i, int64_t j, bool whole, int64_t left, const float (&bias)[VE],
+                                         const typename ln_type<DT>::T (&res)[VE], float (&v)[VE])
 {
     using T = typename ln_type<DT>::T;
-    const bool whole = j + VE <= g.n;
-    T *out = (T *)g.out + i * g.ldo + j;
-    if (g.bias) {
-        const T *bias = (const T *)g.bias + j;
 #pragma unroll
-        for (int u = 0; u < VE; ++u)
-            if (whole || j + u < g.n)
-                v[u] += (float)bias[u];
-    }
-    auto put = [&](T *to) {
-        T o[VE];
-#pragma unroll
-        for (int u = 0; u < VE; ++u)
-            o[u] = (T)v[u];
-        if (whole) {
-            ln_u128 raw;
-            __builtin_memcpy(&raw, o, 16);
-            *reinterpret_cast<ln_u128 *>(to) = raw;
-        } else {
-#pragma unroll
-            for (int u = 0; u < VE; ++u)
-                if (j + u < g.n)
-                    to[u] = o[u];
-        }
-    };
+    for (int u = 0; u < VE; ++u)
+        v[u] += bias[u];
     if (g.preact)
-        put((T *)g.preact + i * g.ldp + j);
-    if (g.act != ACT_NONE)
+        ln_write<DT, VE>((T *)g.preact + i * g.ldp + j, whole, left, v);
 #pragma unroll
-        for (int u = 0; u < VE; ++u)
-            v[u] = ln_act(g.act, v[u]);
-    if (g.residual) {
-        const T *res = (const T *)g.residual + i * g.ldr + j;
-        if (whole) {
-            const ln_u128 raw = *reinterpret_cast<const ln_u128 *>(res);
-            T r[VE];
-            __builtin_memcpy(r, &raw, 16);
-#pragma unroll
-            for (int u = 0; u < VE; ++u)
-                v[u] += (float)r[u];
-        } else {
-#pragma unroll
-            for (int u = 0; u < VE; ++u)
-                if (j + u < g.n)
-                    v[u] += (float)res[u];
-        }
+    for (int u = 0; u < VE; ++u)
+        v[u] = ln_act(act, v[u]) + (float)res[u];
+    ln_write<DT, VE>((T *)g.out + i * g.ldo + j, whole, left, v);
+}
+
+// calls f with the activation as a compile-time constant
+template <typename F>
+__device__ __forceinline__ void ln_with_act(int act, F &&f)
+{
+    switch (act) {
+    case ACT_RELU:
+        return f(std::integral_constant<int, ACT_RELU>());
+    case ACT_GELU:
+        return f(std::integral_constant<int, ACT_GELU>());
+    case ACT_GELU_TANH:
+        return f(std::integral_constant<int, ACT_GELU_TANH>());
+    case ACT_SILU:
+        return f(std::integral_constant<int, ACT_SILU>());
+    case ACT_SIGMOID:
+        return f(std::integral_constant<int, ACT_SIGMOID>());
+    default:
+        return f(std::integral_constant<int, ACT_NONE>());
     }
-    put(out);
 }
 
 constexpr int LN_BK = 128;  // bytes of contraction per stage: one 128-byte line of every operand row
 
-// Tiles of BM x BN, WM x WN waves of (BM / WM) x (BN / WN).  Operands go to LDS directly (16 bytes a lane, 8 rows of 128
-// bytes an instruction), two stages: stage s + 1 is in flight while stage s is multiplied, one barrier a stage.  The
-// 16-byte chunk index of a row is XORed with (row >> 1) & 7 on the source address and on the fragment reads, so that the
-// 32 rows of a fragment read spread over the banks.
-template <int DT, int BM, int BN, int WM, int WN, bool SPLIT>
-__global__ __launch_bounds__(WM *WN * 64) void k_linear(ln_gemm g)
+// Where a workgroup works.  Consecutive workgroups go to the eight XCDs in turn, so that each XCD gets a contiguous run of
+// the tile order, which walks groups of 8 tile rows column by column (their operands stay in the XCD's L2).
+struct ln_place {
+    int64_t row0, col0, s_lo, s_hi;  // the tile's first cell, the stages of the contraction
+    int split;
+};
+template <int BM, int BN, bool SPLIT>
+__device__ __forceinline__ ln_place ln_tile_of(const ln_gemm &g)
+{
+    // (32-bit: the launcher keeps the workgroups below 2^31; 64-bit divisions cost microseconds at the start of every tile)
+    const uint32_t nty = (uint32_t)((g.m + BM - 1) / BM), ntx = (uint32_t)((g.n + BN - 1) / BN), tiles = nty * ntx;
+    const uint32_t bid = blockIdx.x, nwg = gridDim.x, q8 = nwg / 8, r8 = nwg % 8, xcd = bid % 8;
+    const uint32_t seq = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + bid / 8;
+    const uint32_t split = SPLIT ? seq / tiles : 0, tile = SPLIT ? seq - split * tiles : seq;
+    const uint32_t group = tile / (8 * ntx), first = group * 8, rows_in = min(8u, nty - first), in_group = tile - group * 8 * ntx;
+    const uint32_t col = in_group / rows_in;
+    ln_place p;
+    p.row0 = (int64_t)(first + in_group - col * rows_in) * BM;
+    p.col0 = (int64_t)col * BN;
+    p.split = (int)split;
+    p.s_lo = SPLIT ? p.split * g.stages_per_split : 0;
+    p.s_hi = SPLIT ? min(g.stages, p.s_lo + g.stages_per_split) : g.stages;
+    return p;
+}
+
+// A wave's FM x FN sub-tiles of 32 x 32, at (wrow, wcol) of the workgroup's tile.  B is the products' left operand, so that a
+// lane holds cells of one row (row lane % 32, register 4 q + u: column 8 q + 4 (lane / 32) + u); 32 rows at a time go through LDS (this wave's own part of `s_f`) and leave
+// as 16-byte pieces of rows.  The residual's pieces of the next rows are under way while these are worked on: with one wave
+// a SIMD nothing else hides their latency (8192 x 4096 outputs of k = 4096 with silu, residual and pre-activation: 353 us
+// without, 286 with).
+template <int FN>
+constexpr int ln_trow = FN * 32 + 4;  // floats of a buffered row: 16-byte aligned, spread over the banks
+template <int DT, int FM, int FN, bool SPLIT>
+__device__ __forceinline__ void ln_store_tile(const ln_gemm &g, const ln_place &at, const f32x16 (&acc)[FM][FN], float *s_f, int wid, int wrow, int wcol, int lane)
+{
+    using T = typename ln_type<DT>::T;
+    constexpr int TROW = ln_trow<FN>, VE = SPLIT ? 4 : ln_type<DT>::VE, PIECES = FN * 32 / VE, ROWS = 64 / PIECES, PASSES = 32 / ROWS;
+    const int fr = lane & 31, fh = lane >> 5, pr = lane / PIECES, pc = lane % PIECES * VE;
+    float *buf = s_f + wid * 32 * TROW;
+    const int64_t j = at.col0 + wcol + pc, left = g.n - j;
+    auto put = [&](auto A) {
+        constexpr int aa = decltype(A)::value;
+        // (the two comments keep the branches of to_lds apart: merged, they would index the registers at run time, in scratch memory)
+        asm volatile("; rows %0" ::"n"(aa * 32));
+#pragma unroll
+        for (int b = 0; b < FN; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4 *>(buf + fr * TROW + b * 32 + 8 * q + 4 * fh) = make_float4(acc[aa][b][4 * q], acc[aa][b][4 * q + 1], acc[aa][b][4 * q + 2], acc[aa][b][4 * q + 3]);
+        asm volatile("; rows %0 done" ::"n"(aa * 32) : "memory");
+    };
+    auto to_lds = [&](int a) {
+        if constexpr (FM == 4) {
+            if (a == 0)
+                put(std::integral_constant<int, 0>());
+            else if (a == 1)
+                put(std::integral_constant<int, 1>());
+            else if (a == 2)
+                put(std::integral_constant<int, 2>());
+            else
+                put(std::integral_constant<int, 3>());
+        } else if constexpr (FM == 2) {
+            if (a == 0)
+                put(std::integral_constant<int, 0>());
+            else
+                put(std::integral_constant<int, 1>());
+        } else {
+            static_assert(FM == 1, "rows of sub-tiles");
+            put(std::integral_constant<int, 0>());
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    auto from_lds = [&](int p, float (&v)[VE]) {
+#pragma unroll
+        for (int u = 0; u < VE; u += 4) {
+            const float4 f = *reinterpret_cast<const float4 *>(buf + (p * ROWS + pr) * TROW + pc + u);
+            v[u] = f.x;
+            v[u + 1] = f.y;
+            v[u + 2] = f.z;
+            v[u + 3] = f.w;
+        }
+    };
+    constexpr int UNROLL = FM > 2 ? 1 : 64;
+    if constexpr (SPLIT) {
+#pragma unroll UNROLL
+        for (int a = 0; a < FM; ++a) {
+            to_lds(a);
+#pragma unroll
+            for (int p = 0; p < PASSES; ++p) {
+                const int64_t i = at.row0 + wrow + a * 32 + p * ROWS + pr;
+                float v[VE];
+                from_lds(p, v);
+                if (i < g.m && left > 0)
+                    *reinterpret_cast<float4 *>(g.partial + ((int64_t)at.split * g.m + i) * g.ldq + j) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    } else {
+        constexpr int CHUNK = PASSES < 8 ? PASSES : 8, CHUNKS = PASSES / CHUNK;
+        const bool whole = left >= VE;
+        float bias[VE];
+        {
+            T b[VE];
+#pragma unroll
+            for (int u = 0; u < VE; ++u)
+                b[u] = (T)0.0f;
+            if (g.bias && left > 0)
+                ln_read<DT, VE>((const T *)g.bias + j, whole, left, b);
+#pragma unroll
+            for (int u = 0; u < VE; ++u)
+                bias[u] = (float)b[u];
+        }
+        T res[CHUNK][VE], next[CHUNK][VE];
+        auto fetch = [&](int it, T (&r)[CHUNK][VE]) {  // the residual of chunk `it` of FM * CHUNKS
+#pragma unroll
+            for (int p = 0; p < CHUNK; ++p) {
+                const int64_t i = at.row0 + wrow + (it * CHUNK + p) * ROWS + pr;
+                if (g.residual && i < g.m && left > 0)
+                    ln_read<DT, VE>((const T *)g.residual + i * g.ldr + j, whole, left, r[p]);
+                else
+#pragma unroll
+                    for (int u = 0; u < VE; ++u)
+                        r[p][u] = (T)0.0f;
+            }
+        };
+        fetch(0, res);
+#pragma unroll UNROLL  // (the activations' code once per 32 rows of a large tile)
+        for (int it = 0; it < FM * CHUNKS; ++it) {
+            const int c = it % CHUNKS;
+            if (c == 0)
+                to_lds(it / CHUNKS);
+            if (g.residual && it + 1 < FM * CHUNKS)
+                fetch(it + 1, next);
+            ln_with_act(g.act, [&](auto ACT) {
+#pragma unroll
+                for (int p = 0; p < CHUNK; ++p) {
+                    const int64_t i = at.row0 + wrow + (it * CHUNK + p) * ROWS + pr;
+                    float v[VE];
+                    from_lds(c * CHUNK + p, v);
+                    if (i < g.m && left > 0)
+                        ln_cells<DT, VE>(g, decltype(ACT)::value, i, j, whole, left, bias, res[p], v);
+                }
+            });
+            if (g.residual)
+#pragma unroll
+                for (int p = 0; p < CHUNK; ++p)
+#pragma unroll
+                    for (int u = 0; u < VE; ++u)
+                        res[p][u] = next[p][u];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    }
+}
+
+// Tiles of BM x BN, 2 x 2 waves of (BM / 2) x (BN / 2).  Operands go to LDS directly (16 bytes a lane, 8 rows of 128 bytes an
+// instruction), in stages of 128 bytes of contraction: A(0), B(0), A(1), B(1), ... through a ring of five slots, so that two
+// and a half stages are held.  The 16-byte chunk index of a row is XORed with (row >> 1) & 7 on the source address and on the
+// fragment reads, so that the 32 rows of a fragment read spread over the banks.
+//
+// A wave keeps its matrix unit fed by itself: while the FM x FN products of a 32-byte step run, the fragments of the next
+// step are read into the other of two register sets and a quarter of a stage is fetched, one instruction at a time between
+// the products.  One barrier a stage, before its last step: by then everybody has read the stage (its slots are free) and the
+// next stage has landed (its first fragments are read during the last step).  In stage s the steps fetch the second half of
+// B(s+1), A(s+2), and after the barrier the first half of B(s+2): what is fetched has two steps or more to arrive, and all
+// four steps load the memory pipe alike.  bfloat16, 256 x 256 tiles, all compute units busy: 1.46 us a stage; with two whole
+// stages in memory, fetching in two of the steps 1.59, in one of them 1.66, all between the barriers of a simpler loop 1.8.
+template <int DT, int BM, int BN, bool SPLIT, typename OFF = uint32_t>
+__global__ __launch_bounds__(256, (BM + BN) > 256 ? 1 : 2) void k_linear(ln_gemm g)
 {
     using P = ln_type<DT>;
     using V = typename P::V;
-    constexpr int NWAVE = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
-    constexpr int STAGE = (BM + BN) * LN_BK, PER_WAVE = (BM + BN) / 8 / NWAVE;
-    constexpr int TROW = TN + 4;  // floats of a buffered output row: 16-byte aligned, spread over the banks
-    static_assert((BM + BN) % (8 * NWAVE) == 0 && TM % 32 == 0 && TN % 32 == 0, "tile");
-    static_assert(NWAVE * 32 * TROW * 4 <= 2 * STAGE, "the epilogue reuses the stages' memory");
-    __shared__ __attribute__((aligned(16))) uint8_t s_t[2 * STAGE];
+    constexpr int TM = BM / 2, TN = BN / 2, FM = TM / 32, FN = TN / 32, KS = LN_BK / 32, RING = 5;
+    constexpr int NA = BM / 32, NB = BN / 32;  // fetches of a wave for an operand's stage
+    constexpr int SLOT = (BM > BN ? BM : BN) * LN_BK;
+    static_assert(NA % 2 == 0 && NB % 2 == 0 && TM % 32 == 0 && TN % 32 == 0 && KS == 4, "tile");
+    static_assert(4 * 32 * ln_trow<FN> * 4 <= RING * SLOT && RING * SLOT <= 160 * 1024, "memory");
+    __shared__ __attribute__((aligned(16))) uint8_t s_t[RING * SLOT];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const ln_place at = ln_tile_of<BM, BN, SPLIT>(g);
+    const int64_t row0 = at.row0, col0 = at.col0, s_lo = at.s_lo, s_hi = at.s_hi, kbytes = g.k * (int64_t)sizeof(typename P::T);
 
-    // tile of this workgroup: consecutive workgroups go to the eight XCDs in turn, so that each XCD gets a contiguous run
-    // of the tile order, which walks groups of 8 tile rows column by column (their operands stay in the XCD's L2)
-    const int64_t nty = (g.m + BM - 1) / BM, ntx = (g.n + BN - 1) / BN, tiles = nty * ntx;
-    const int64_t bid = blockIdx.x, nwg = gridDim.x, q8 = nwg / 8, r8 = nwg % 8, xcd = bid % 8;
-    const int64_t seq = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + bid / 8;
-    const int64_t tile = SPLIT ? seq % tiles : seq;
-    const int split = SPLIT ? (int)(seq / tiles) : 0;
-    const int64_t group = tile / (8 * ntx), first = group * 8, rows_in = min((int64_t)8, nty - first), in_group = tile - group * 8 * ntx;
-    const int64_t row0 = (first + in_group % rows_in) * BM, col0 = in_group / rows_in * BN;
-
-    const int64_t kbytes = g.k * (int64_t)sizeof(typename P::T);
-    const int64_t nst_all = (kbytes + LN_BK - 1) / LN_BK;
-    const int64_t s_lo = SPLIT ? split * g.stages_per_split : 0, s_hi = SPLIT ? min(nst_all, s_lo + g.stages_per_split) : nst_all;
-
-    // staging: instruction q of wave w lands rows [8 (w PER_WAVE + q), + 8) of the stage (A's rows first, then B's)
+    // instruction q of wave w lands rows [8 (w NA + q), + 8) of A's stage, or B's.  OFF is 64-bit where a tile's rows may span
+    // 2^32 bytes.
+    const uint8_t *const a0 = g.a + row0 * g.lda, *const b0 = g.b + col0 * g.ldb;
     const int srow = lane >> 3, schunk = lane & 7;
-    const uint8_t *src[PER_WAVE];
-    int skb[PER_WAVE];
+    OFF offa[NA], offb[NB];
+    auto chunk_of = [&](int r) { return (schunk ^ ((r >> 1) & 7)) * 16; };
 #pragma unroll
-    for (int q = 0; q < PER_WAVE; ++q) {
-        const int r = (wid * PER_WAVE + q) * 8 + srow;
-        const bool is_a = (wid * PER_WAVE + q) * 8 < BM;
-        const int64_t at = is_a ? min(row0 + r, g.m - 1) : min(col0 + (r - BM), g.n - 1);  // rows past the end: any, not stored
-        skb[q] = (schunk ^ ((r >> 1) & 7)) * 16;
-        src[q] = (is_a ? g.a + at * g.lda : g.b + at * g.ldb) + skb[q];
+    for (int q = 0; q < NA; ++q) {
+        const int r = (wid * NA + q) * 8 + srow;
+        offa[q] = (OFF)(min((int64_t)r, g.m - 1 - row0) * g.lda) + (OFF)chunk_of(r);  // rows past the end: any, not stored
     }
-    auto stage = [&](int64_t s) {
-        uint8_t *to = s_t + (int)(s & 1) * STAGE + wid * PER_WAVE * 8 * LN_BK;
-        const int64_t k0 = s * LN_BK;
-        const bool whole = k0 + LN_BK <= kbytes;
 #pragma unroll
-        for (int q = 0; q < PER_WAVE; ++q) {
-            const uint8_t *p = src[q] + k0;
-            if (!whole && k0 + skb[q] >= kbytes)
+    for (int q = 0; q < NB; ++q) {
+        const int r = (wid * NB + q) * 8 + srow;
+        offb[q] = (OFF)(min((int64_t)r, g.n - 1 - col0) * g.ldb) + (OFF)chunk_of(r);
+    }
+    const int64_t last = kbytes % LN_BK ? kbytes / LN_BK : -1;  // the stage that the contraction ends in, if it does not fill it
+    auto fetch = [&](auto WHOLE, bool is_a, int64_t s, int q, int slot) {
+        const int r8 = (wid * (is_a ? NA : NB) + q) * 8;
+        const uint8_t *p = (is_a ? a0 + offa[is_a ? q : 0] : b0 + offb[is_a ? 0 : q]) + s * LN_BK;
+        if (!decltype(WHOLE)::value)
+            if (s == last && s * LN_BK + chunk_of(r8 + srow) >= kbytes)
                 p = reinterpret_cast<const uint8_t *>(&ln_zero_block);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)p, (__attribute__((address_space(3))) void *)(to + q * 8 * LN_BK), 16, 0, 0);
-        }
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)p, (__attribute__((address_space(3))) void *)(s_t + slot + r8 * LN_BK), 16, 0, 0);
+    };
+    auto fwd = [](int slot, int by) {  // `by` slots on
+        slot += by * SLOT;
+        return slot >= RING * SLOT ? slot - RING * SLOT : slot;
     };
 
     f32x16 acc[FM][FN];
@@ -251,84 +418,121 @@ __global__ __launch_bounds__(WM *WN * 64) void k_linear(ln_gemm g)
             for (int r = 0; r < 16; ++r)
                 acc[a][b][r] = 0.0f;
 
-    const int fr = lane & 31, fh = lane >> 5, wr = wid / WN, wc = wid % WN;
-    if (s_lo < s_hi)
-        stage(s_lo);
-    for (int64_t s = s_lo; s < s_hi; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of stage s has landed
-        __builtin_amdgcn_s_barrier();                     // everybody's has, and everybody has read stage s - 1
+    const int fr = lane & 31, fh = lane >> 5, wr = wid >> 1, wc = wid & 1;
+    V fa[2][FM], fb[2][FN];
+    // (the waves' rows are multiples of 16: the XOR of every row of a fragment is that of fr)
+    const int swz = (fr >> 1) & 7;
+    const uint8_t *const la = s_t + (wr * TM + fr) * LN_BK, *const lb = s_t + (wc * TN + fr) * LN_BK;
+    auto frag = [&](auto SET, int slot, int ks, int i) {  // the i-th of FM + FN fragments of step ks of the stage whose A is at `slot`
+        constexpr int set = decltype(SET)::value;
+        const int c = ((ks * 2 + fh) ^ swz) * 16;
+        if (i < FM)
+            fa[set][i] = *reinterpret_cast<const V *>(la + slot + c + i * 32 * LN_BK);
+        else
+            fb[set][i - FM] = *reinterpret_cast<const V *>(lb + fwd(slot, 1) + c + (i - FM) * 32 * LN_BK);
+    };
+    using S0 = std::integral_constant<int, 0>;
+    using S1 = std::integral_constant<int, 1>;
+    // the products of set SET; between them the fragments of step `ks` (of the stage at `slot`) into the other set and half of the
+    // fetches of an operand's stage `sf`, from the q0-th on, into slot `to`
+    auto step = [&](auto SET, auto WHOLE, bool reading, int slot, int ks, bool fetching, auto IS_A, int64_t sf, int q0, int to) {
+        constexpr int set = decltype(SET)::value;
+        using OTHER = std::integral_constant<int, 1 - set>;
+        constexpr bool is_a = decltype(IS_A)::value;
+        // (parts outside: no product waits for the one before it)
+        constexpr int NP = FM * FN, NT = NP * P::PARTS, NR = FM + FN, HALF = (is_a ? NA : NB) / 2;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int a = t % NP / FN, b = t % NP % FN;
+#pragma unroll
+            for (int i = t * NR / NT; i < (t + 1) * NR / NT; ++i)
+                if (reading)
+                    frag(OTHER(), slot, ks, i);
+            acc[a][b] = P::mfma(fb[set][b], fa[set][a], acc[a][b], t / NP);
+#pragma unroll
+            for (int q = t * HALF / NT; q < (t + 1) * HALF / NT; ++q)
+                if (fetching)
+                    fetch(WHOLE, is_a, sf, q0 + q, to);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    using OF_A = std::true_type;
+    using OF_B = std::false_type;
+    // stage s, its A at `slot`; WHOLE: stages s + 1 and s + 2 exist and are filled by the contraction
+    auto body = [&](auto WHOLE, int64_t s, int slot) {
+        constexpr bool whole = decltype(WHOLE)::value;
+        const bool more = whole || s + 1 < s_hi, more2 = whole || s + 2 < s_hi;
+        step(S0(), WHOLE, true, slot, 1, more, OF_B(), s + 1, NB / 2, fwd(slot, 3));
+        step(S1(), WHOLE, true, slot, 2, more2, OF_A(), s + 2, 0, fwd(slot, 4));
+        step(S0(), WHOLE, true, slot, 3, more2, OF_A(), s + 2, NA / 2, fwd(slot, 4));
+        // this wave has read stage s, and its part of s + 1 has landed (A(s+2), the last NA fetches, may be under way)
+        if (more2)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NA) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 1 < s_hi)
-            stage(s + 1);
-        const uint8_t *sa = s_t + (int)(s & 1) * STAGE, *sb = sa + BM * LN_BK;
-#pragma unroll
-        for (int ks = 0; ks < LN_BK / 32; ++ks) {
-            V fa[FM], fb[FN];
-#pragma unroll
-            for (int t = 0; t < FM; ++t) {
-                const int r = wr * TM + t * 32 + fr;
-                fa[t] = *reinterpret_cast<const V *>(sa + r * LN_BK + (((ks * 2 + fh) ^ ((r >> 1) & 7)) * 16));
-            }
-#pragma unroll
-            for (int t = 0; t < FN; ++t) {
-                const int r = wc * TN + t * 32 + fr;  // (BM is a multiple of 16: the XOR of row BM + r is that of r)
-                fb[t] = *reinterpret_cast<const V *>(sb + r * LN_BK + (((ks * 2 + fh) ^ ((r >> 1) & 7)) * 16));
-            }
-#pragma unroll
-            for (int a = 0; a < FM; ++a)
-#pragma unroll
-                for (int b = 0; b < FN; ++b)
-                    acc[a][b] = P::mfma(fa[a], fb[b], acc[a][b]);
-        }
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __syncthreads();  // the stages have been read: their memory buffers the output
+        step(S1(), WHOLE, more, fwd(slot, 2), 0, more2, OF_B(), s + 2, 0, slot);
+    };
 
-    // A lane holds one column of a 32 x 32 sub-tile (register 4 q + u: row 8 q + 4 (lane / 32) + u).  32 rows at a time go
-    // through LDS (this wave's own part) and leave as 16-byte pieces of rows.
-    float *buf = reinterpret_cast<float *>(s_t) + wid * 32 * TROW;
+    if (s_lo < s_hi) {
+        using ANY = std::false_type;
 #pragma unroll
-    for (int a = 0; a < FM; ++a) {
+        for (int q = 0; q < NA; ++q)
+            fetch(ANY(), true, s_lo, q, 0);
 #pragma unroll
-        for (int b = 0; b < FN; ++b)
+        for (int q = 0; q < NB; ++q)
+            fetch(ANY(), false, s_lo, q, SLOT);
+        if (s_lo + 1 < s_hi) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                buf[(8 * (r >> 2) + 4 * fh + (r & 3)) * TROW + b * 32 + fr] = acc[a][b][r];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        constexpr int VE = SPLIT ? 4 : P::VE, PIECES = TN / VE, ROWS = 64 / PIECES;
-        const int pr = lane / PIECES, pc = lane % PIECES * VE;
-        const int64_t j = col0 + wc * TN + pc;
-#pragma unroll 1  // (the six activations' code once per 32 rows)
-        for (int p = 0; p < 32 / ROWS; ++p) {
-            const int64_t i = row0 + wr * TM + a * 32 + p * ROWS + pr;
-            float v[VE];
-#pragma unroll
-            for (int u = 0; u < VE; ++u)
-                v[u] = buf[(p * ROWS + pr) * TROW + pc + u];
-            if (i < g.m && j < g.n) {
-                if constexpr (SPLIT) {
-                    *reinterpret_cast<float4 *>(g.partial + ((int64_t)split * g.m + i) * g.ldq + j) = make_float4(v[0], v[1], v[2], v[3]);
-                } else {
-                    ln_finish<DT, VE>(g, i, j, v);
-                }
-            }
+            for (int q = 0; q < NA; ++q)
+                fetch(ANY(), true, s_lo + 1, q, 2 * SLOT);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NA) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s_lo + 1 < s_hi)
+#pragma unroll
+            for (int q = 0; q < NB / 2; ++q)
+                fetch(ANY(), false, s_lo + 1, q, 3 * SLOT);
+#pragma unroll
+        for (int i = 0; i < FM + FN; ++i)
+            frag(S0(), 0, 0, i);
+        const int64_t s_fast = min(s_hi, last < 0 ? s_hi : last) - 2;
+        int64_t s = s_lo;
+        int slot = 0;
+        for (; s < s_fast; ++s, slot = fwd(slot, 2))
+            body(std::true_type(), s, slot);
+        for (; s < s_hi; ++s, slot = fwd(slot, 2))
+            body(ANY(), s, slot);
     }
+    __syncthreads();  // the stages have been read: their memory buffers the output
+    ln_store_tile<DT, FM, FN, SPLIT>(g, at, acc, reinterpret_cast<float *>(s_t), wid, wr * TM, wc * TN, lane);
 }
 
 // the sums over the splits, in order, and the epilogue
 template <int DT>
 __global__ __launch_bounds__(256) void k_linear_join(ln_gemm g)
 {
+    using T = typename ln_type<DT>::T;
     constexpr int VE = ln_type<DT>::VE;
     const int64_t per_row = (g.n + VE - 1) / VE, total = g.m * per_row;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-        const int64_t i = t / per_row, j = (t - i * per_row) * VE;
-        float v[VE];
+        const int64_t i = t / per_row, j = (t - i * per_row) * VE, left = g.n - j;
+        const bool whole = left >= VE;
+        T b[VE], res[VE];
+        float v[VE], bias[VE];
 #pragma unroll
-        for (int u = 0; u < VE; ++u)
+        for (int u = 0; u < VE; ++u) {
             v[u] = 0.0f;
+            b[u] = res[u] = (T)0.0f;
+        }
+        if (g.bias)
+            ln_read<DT, VE>((const T *)g.bias + j, whole, left, b);
+        if (g.residual)
+            ln_read<DT, VE>((const T *)g.residual + i * g.ldr + j, whole, left, res);
         for (int s = 0; s < g.nsplit; ++s) {
             const float *from = g.partial + ((int64_t)s * g.m + i) * g.ldq + j;
 #pragma unroll
@@ -342,7 +546,10 @@ __global__ __launch_bounds__(256) void k_linear_join(ln_gemm g)
                 }
             }
         }
-        ln_finish<DT, VE>(g, i, j, v);
+#pragma unroll
+        for (int u = 0; u < VE; ++u)
+            bias[u] = (float)b[u];
+        ln_with_act(g.act, [&](auto ACT) { ln_cells<DT, VE>(g, decltype(ACT)::value, i, j, whole, left, bias, res, v); });
     }
 }
 
@@ -489,16 +696,67 @@ __global__ __launch_bounds__(256) void k_linear_bias_grad(int64_t parts, int64_t
 // ---------------------------------------------------------------------------- host side
 constexpr size_t elem_bytes(int dtype) { return dtype == 0 ? 4 : 2; }
 
-template <int DT, int BM, int BN, int WM, int WN>
+template <int DT, int BM, int BN, typename OFF = uint32_t>
 int launch_tiles(skm_ctx *ctx, const ln_gemm &g)
 {
     const int64_t tiles = skm_ceil_div(g.m, BM) * skm_ceil_div(g.n, BN);
     SKM_REQUIRE(tiles * g.nsplit < ((int64_t)1 << 31), SKM_E_OVERFLOW, "skm_linear: too many tiles");
     if (g.nsplit > 1)
-        k_linear<DT, BM, BN, WM, WN, true><<<(unsigned)(tiles * g.nsplit), WM * WN * 64, 0, ctx->stream>>>(g);
+        k_linear<DT, BM, BN, true, OFF><<<(unsigned)(tiles * g.nsplit), 256, 0, ctx->stream>>>(g);
     else
-        k_linear<DT, BM, BN, WM, WN, false><<<(unsigned)tiles, WM * WN * 64, 0, ctx->stream>>>(g);
+        k_linear<DT, BM, BN, false, OFF><<<(unsigned)tiles, 256, 0, ctx->stream>>>(g);
     return skm_check_launch("k_linear");
+}
+
+// What a workgroup of each tile costs, in microseconds measured on MI355X: a 128-byte stage of the contraction with the chip
+// idle around it, the same with every compute unit busy (then the clock, held down by the chip's power, and what the units
+// share bound it), and the rest of the tile (first fetch, epilogue).  16-bit types / float32 (bound by its matrix rate).
+// The plan with the least estimate is taken; e.g. k = 6592 (16 bits), m x n = 3383 x 1000, measured in all: 256 x 256 in 4 parts 58,
+// 256 x 128 in 2 parts 53, 128 x 128 59, 128 x 64 57, 64 x 64 74; 512 x 512, k = 4096: 26 / 19 / 16 / 14 / 12 at the best number of
+// parts of each; 4096 x 4096, k = 4096: 108 / 133 / 151 / 192 / 208; float32 10000 x 1000, k = 6564: 1515 / 1533 / 1186 / 1089 / 1108.
+struct ln_tile {
+    int bm, bn;
+    float idle[2], busy[2], rest;
+};
+const ln_tile LN_TILES[] = {
+    {256, 256, {1.03f, 7.2f}, {1.44f, 8.5f}, 10.0f},
+    {256, 128, {0.53f, 3.7f}, {0.75f, 4.15f}, 5.0f},
+    {128, 128, {0.29f, 1.9f}, {0.53f, 2.0f}, 1.5f},
+    {128, 64, {0.21f, 1.0f}, {0.30f, 1.02f}, 1.2f},
+    {64, 64, {0.16f, 0.54f}, {0.20f, 0.54f}, 0.7f},
+};
+
+struct ln_plan {
+    int tile = 2, nsplit = 1;
+    int64_t stages_per_split = 0;
+};
+
+ln_plan plan_of(int dtype, int64_t cus, int64_t m, int64_t n, int64_t stages)
+{
+    ln_plan best;
+    double best_us = 1e300;
+    const int kind = dtype == 0;
+    for (int t = 0; t < 5; ++t) {
+        const ln_tile &c = LN_TILES[t];
+        const int64_t tiles = skm_ceil_div(m, c.bm) * skm_ceil_div(n, c.bn);
+        for (int64_t want = 1; want <= 32; ++want) {
+            const int64_t per = std::max<int64_t>(skm_ceil_div(stages, want), 1), parts = std::max<int64_t>(skm_ceil_div(stages, per), 1);
+            if (parts != want || (want > 1 && (per < 4 || tiles * want > 4 * cus)))
+                continue;
+            const double blocks = (double)tiles * want, load = std::min(1.0, blocks / (double)cus);
+            const double stage = c.idle[kind] + (c.busy[kind] - c.idle[kind]) * load;
+            double us = (double)skm_ceil_div((int64_t)blocks, cus) * ((double)per * stage + c.rest);
+            if (want > 1)  // the parts' sums travel through the caches, and a second kernel starts
+                us += 4.0 + 8.0 * (double)want * (double)m * (double)n / 12e6;
+            if (us < best_us) {
+                best_us = us;
+                best.tile = t;
+                best.nsplit = (int)want;
+                best.stages_per_split = per;
+            }
+        }
+    }
+    return best;
 }
 
 // C = A B^T with the epilogue; a and b are ready (16-byte rows).
@@ -506,20 +764,11 @@ template <int DT>
 int gemm(skm_ctx *ctx, ln_gemm g)
 {
     const int64_t stages = skm_ceil_div(g.k * (int64_t)elem_bytes(DT), LN_BK);
-    const int64_t big = skm_ceil_div(g.m, 256) * skm_ceil_div(g.n, 256), small = skm_ceil_div(g.m, 128) * skm_ceil_div(g.n, 128);
-    const int64_t cus = ctx->usable_cus;
-    g.nsplit = 1;
-    g.stages_per_split = stages;
-    const bool large = big >= cus;
-    const int64_t tiles = large ? big : small;
-    if (tiles < cus) {
-        int64_t s = std::min<int64_t>(skm_ceil_div(cus * 2, tiles), stages / 4);
-        s = std::min<int64_t>(s, 64);
-        if (s > 1) {
-            g.stages_per_split = skm_ceil_div(stages, s);
-            g.nsplit = (int)skm_ceil_div(stages, g.stages_per_split);
-        }
-    }
+    ln_plan plan = plan_of(DT, ctx->usable_cus, g.m, g.n, stages);
+    const bool wide = std::max(g.lda, g.ldb) >= ((int64_t)1 << 24);  // 256 rows may span 2^32 bytes
+    g.stages = stages;
+    g.nsplit = plan.nsplit;
+    g.stages_per_split = plan.stages_per_split;
     if (g.nsplit > 1) {
         void *p;
         g.ldq = skm_ceil_div(g.n, 4) * 4;
@@ -528,10 +777,18 @@ int gemm(skm_ctx *ctx, ln_gemm g)
     }
     {
         SKM_PROF(ctx, "k_linear");
-        if (large)
-            SKM_TRY((launch_tiles<DT, 256, 256, 2, 4>(ctx, g)));
+        if (wide)
+            SKM_TRY((launch_tiles<DT, 128, 128, uint64_t>(ctx, g)));
+        else if (plan.tile == 0)
+            SKM_TRY((launch_tiles<DT, 256, 256>(ctx, g)));
+        else if (plan.tile == 1)
+            SKM_TRY((launch_tiles<DT, 256, 128>(ctx, g)));
+        else if (plan.tile == 2)
+            SKM_TRY((launch_tiles<DT, 128, 128>(ctx, g)));
+        else if (plan.tile == 3)
+            SKM_TRY((launch_tiles<DT, 128, 64>(ctx, g)));
         else
-            SKM_TRY((launch_tiles<DT, 128, 128, 2, 2>(ctx, g)));
+            SKM_TRY((launch_tiles<DT, 64, 64>(ctx, g)));
     }
     if (g.nsplit > 1) {
         SKM_PROF(ctx, "k_linear_join");
