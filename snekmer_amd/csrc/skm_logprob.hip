@@ -17,9 +17,13 @@
 // and the running list of the k best.  Rows with many tiles are shared by the waves of a workgroup, few long rows by
 // several workgroups whose partial states a second kernel joins.
 //
-// The k best of a tile: no element below the k-th largest of the 64 lane maxima can be among them, so only those above
-// it (about as many as k) are collected in LDS and ranked; equal ones are taken in index order until k are held.  After
-// the first tile only elements above the list's last one are looked at, which costs one comparison a tile.
+// The k best of a tile: its lanes form G groups (G the power of two from k on), and no element below the k-th largest of the
+// group maxima can be among them, so only those above it (hardly more than k) are collected in LDS and ranked; equal ones
+// are taken in index order until k are held.  After the first tile only elements above the list's last one are looked at,
+// which costs one comparison a tile.
+//
+// Many short rows (the learn / apply block) are bound by instructions, not by memory: a wave takes up to eight rows, holds
+// row r's state in lane r, and does logarithms, divisions and label look-ups for all of them at once.
 #include <algorithm>
 #include <cmath>
 
@@ -30,7 +34,7 @@ namespace {
 constexpr int LP_E = 16;            // scores a lane holds of a tile
 constexpr int LP_TILE = 64 * LP_E;  // 1024
 constexpr int LP_KMAX = 16;
-constexpr int LP_BUF = 128;  // candidates a wave holds before it ranks them (after ranking: at most 16, and 64 may follow)
+constexpr int LP_BUF = 64 + LP_TILE / 2 + 2 * LP_KMAX;  // candidates a wave can hold: 64, half a tile, and the list that comes of them
 constexpr int LP_MAX_SPLITS = 64;
 constexpr float LP_INF = __builtin_inff();
 
@@ -51,7 +55,7 @@ struct lp_args {
     int nsplit;
     int64_t tiles_per_split;
     float4 *part;       // [rows][nsplit]: m, S, Q, c (negative: a score that has no distribution)
-    uint64_t *part_keys;  // [rows][nsplit][LP_KMAX]
+    uint2 *part_lists;  // [rows][nsplit][LP_KMAX]: (score, index), index 0xFFFFFFFF behind the last
 };
 
 // ---- wave helpers: results uniform over the wave
@@ -83,6 +87,10 @@ __device__ __forceinline__ float lp_wave_max(float v)
 __device__ __forceinline__ float lp_wave_sum(float v)
 {
     return __uint_as_float(lp_reduce(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+__device__ __forceinline__ float lp_wave_min(float v)
+{
+    return __uint_as_float(lp_reduce(__float_as_uint(v), 0x7F800000u, [](uint32_t a, uint32_t b) { return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b))); }));
 }
 __device__ __forceinline__ uint32_t lp_wave_umax(uint32_t v)
 {
@@ -154,60 +162,96 @@ struct lp_type<2> {
     static __device__ __forceinline__ T round(float v) { return (__bf16)v; }
 };
 
-// One tile of a row: x[v * VE + u] = score of class base + (v * 64 + lane) * VE + u, -inf where masked or past the end.
-// MASK: 0 none, 1 present.
+// One tile of a row on its way: vector v of a lane holds classes (v * 64 + lane) * VE .. of the tile.
 template <int DT, int MASK>
-__device__ __forceinline__ void lp_load_tile(const typename lp_type<DT>::T *row, const uint8_t *mrow, int64_t base, int64_t cols, int lane, float (&x)[LP_E])
+struct lp_raw {
+    static constexpr int VE = lp_type<DT>::VE, NV = LP_E / VE;
+    lp_u128 v[NV];
+    uint32_t mask[MASK ? NV : 1][VE / 4];
+};
+
+// Where vector v of a lane starts in a tile of which `rem` classes are left: vectors that would reach past the row's end
+// start earlier, at its last whole vector (their first elements, which another lane holds, are dropped in lp_unpack): all
+// loads are whole, unconditional and inside the row.
+template <int VE>
+__device__ __forceinline__ int lp_start(int v, int lane, int rem)
 {
-    using P = lp_type<DT>;
-    constexpr int VE = P::VE, NV = LP_E / VE;
-    if (base + LP_TILE <= cols) {
-        lp_u128 raw[NV];
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-            raw[v] = *reinterpret_cast<const lp_u128 *>(row + base + (v * 64 + lane) * VE);
-        uint32_t mk[NV][VE / 4];
-        if (MASK) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const uint8_t *at = mrow + base + (v * 64 + lane) * VE;
-                if constexpr (VE == 4) {
-                    mk[v][0] = reinterpret_cast<const lp_u32 *>(at)->w[0];
-                } else {
-                    const lp_u64 w = *reinterpret_cast<const lp_u64 *>(at);
-                    mk[v][0] = w.w[0];
-                    mk[v][1] = w.w[1];
-                }
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int u = 0; u < VE; ++u) {
-                float f = P::pick(raw[v], u);
-                if (MASK)
-                    f = ((mk[v][u >> 2] >> (8 * (u & 3))) & 0xFFu) ? f : -LP_INF;
-                x[v * VE + u] = f;
-            }
-    } else {
+    return min((v * 64 + lane) * VE, rem - VE);
+}
+
+// at, mat: the tile's first score and mask byte; rem <= LP_TILE classes are left there; the row has `cols`
+template <int DT, int MASK>
+__device__ __forceinline__ void lp_fetch(const typename lp_type<DT>::T *at, const uint8_t *mat, int rem, int64_t cols, int lane, lp_raw<DT, MASK> &raw)
+{
+    using T = typename lp_type<DT>::T;
+    constexpr int VE = lp_raw<DT, MASK>::VE, NV = lp_raw<DT, MASK>::NV;
+    if (cols >= VE) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int64_t at = base + (v * 64 + lane) * VE;
-            if (at + VE <= cols) {
-                const lp_u128 raw = *reinterpret_cast<const lp_u128 *>(row + at);
+            const int off = lp_start<VE>(v, lane, rem);
+            raw.v[v] = *reinterpret_cast<const lp_u128 *>(at + off);
+            if constexpr (MASK && VE == 4) {
+                raw.mask[v][0] = reinterpret_cast<const lp_u32 *>(mat + off)->w[0];
+            } else if constexpr (MASK) {
+                const lp_u64 w = *reinterpret_cast<const lp_u64 *>(mat + off);
+                raw.mask[v][0] = w.w[0];
+                raw.mask[v][1] = w.w[1];
+            }
+        }
+    } else {  // rows shorter than a vector: as the last elements of one
+        T one[VE];
+        uint8_t m[VE];
+#pragma unroll
+        for (int u = 0; u < VE; ++u) {
+            const int j = u - (VE - rem);
+            one[u] = j >= 0 ? at[j] : (T)0.0f;
+            m[u] = MASK && j >= 0 ? mat[j] : 0;
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            __builtin_memcpy(&raw.v[v], one, 16);
+            if (MASK)
+                __builtin_memcpy(raw.mask[v], m, VE);
+        }
+    }
+}
+
+// x[v * VE + u] = the score at lp_start(v) + u, -inf where masked, past the end or held by another lane
+template <int DT, int MASK>
+__device__ __forceinline__ void lp_unpack(lp_raw<DT, MASK> raw, int rem, int lane, float (&x)[LP_E])
+{
+    constexpr int VE = lp_raw<DT, MASK>::VE, NV = lp_raw<DT, MASK>::NV;
+    // (words that the compiler cannot look into: it would cut the 16-byte loads into the pieces that are used)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        asm volatile("" : "+v"(raw.v[v].w[0]), "+v"(raw.v[v].w[1]), "+v"(raw.v[v].w[2]), "+v"(raw.v[v].w[3]));
+        if (MASK)
+#pragma unroll
+            for (int h = 0; h < VE / 4; ++h)
+                asm volatile("" : "+v"(raw.mask[v][h]));
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int u = 0; u < VE; ++u) {
+            float f = lp_type<DT>::pick(raw.v[v], u);
+            if (MASK)
+                f = ((raw.mask[v][u >> 2] >> (8 * (u & 3))) & 0xFFu) ? f : -LP_INF;
+            x[v * VE + u] = f;
+        }
+    if (rem < LP_TILE) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int drop = (v * 64 + lane) * VE - lp_start<VE>(v, lane, rem);
+            if (rem % VE == 0) {  // (all or none of a vector)
 #pragma unroll
                 for (int u = 0; u < VE; ++u)
-                    x[v * VE + u] = P::pick(raw, u);
+                    x[v * VE + u] = drop > 0 ? -LP_INF : x[v * VE + u];
             } else {
 #pragma unroll
                 for (int u = 0; u < VE; ++u)
-                    x[v * VE + u] = at + u < cols ? P::one(row[at + u]) : -LP_INF;
+                    x[v * VE + u] = u < drop ? -LP_INF : x[v * VE + u];
             }
-            if (MASK)
-#pragma unroll
-                for (int u = 0; u < VE; ++u)
-                    if (at + u < cols && mrow[at + u] == 0)
-                        x[v * VE + u] = -LP_INF;
         }
     }
 }
@@ -222,109 +266,220 @@ struct lp_state {
     float tau = -LP_INF;  // the score of the last of k
 };
 
-// The n candidates of the buffer, best first; the first k stay.
-__device__ __forceinline__ void lp_rank(uint64_t *buf, int n, int k, int lane, lp_state &st)
+// The n candidates of the buffer as (score, index), of which the first st.len are the sorted list so far: ranked, the best k
+// stay.  TIES: equal scores are to be expected (16-bit types).
+template <bool TIES>
+__device__ __forceinline__ void lp_rank(uint2 *buf, int n, int k, int lane, lp_state &st)
 {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const uint64_t a = lane < n ? buf[lane] : 0, b = lane + 64 < n ? buf[lane + 64] : 0;
-    int ra = 0, rb = 0;
-    const int first = n < 64 ? n : 64;
-    for (int j = 0; j < first; ++j) {
-        const uint64_t s = lp_readlane64(a, j);
-        ra += s > a;
-        rb += s > b;
+    if (n <= 64) {  // a lane a candidate
+        const uint2 q = buf[lane];
+        const uint64_t key = lane < n ? lp_key(__uint_as_float(q.x), q.y) : 0;
+        int rank = 0;
+        bool done = false;
+        if (st.len == k) {  // a full list and some that may enter it: only those are compared with everybody
+            rank = lane < k ? lane : 0;
+            for (int j = k; j < n; ++j) {
+                const uint64_t s = lp_readlane64(key, j);
+                rank += s > key;
+                const int behind = __popcll(__ballot(lane < k && key > s));  // (of the list, ahead of candidate j)
+                rank += lane == j ? behind : 0;
+            }
+            done = true;
+        } else if (!TIES) {
+            const float v = lane < n ? __uint_as_float(q.x) : -LP_INF;
+            for (int j = 0; j < n; j += 4)  // (lanes past the end hold -inf)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    rank += __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(v), j + i)) > v;
+            const bool mine = lane < n && rank < k;
+            if (mine)
+                buf[rank] = q;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            done = __ballot(mine && buf[rank].y != q.y) == 0;  // (else equal scores met in one place)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        if (!done) {
+            rank = 0;
+            for (int j = 0; j < n; ++j)
+                rank += lp_readlane64(key, j) > key;
+        }
+        if (lane < n && rank < k)
+            buf[rank] = q;
+    } else {  // (rows in rising order, scores that are nearly all equal) one after the other
+        uint2 *out = buf + n;  // (n + k stays below the buffer's end: see lp_collect)
+#pragma unroll 1
+        for (int r = 0; r < k; ++r) {
+            uint64_t best = 0;
+            int which = 0;
+            for (int i = lane; i < n; i += 64) {
+                const uint2 q = buf[i];
+                const uint64_t a = q.y != 0xFFFFFFFFu ? lp_key(__uint_as_float(q.x), q.y) : 0;
+                which = a > best ? i : which;
+                best = a > best ? a : best;
+            }
+            const uint32_t hi = lp_wave_umax((uint32_t)(best >> 32));
+            const uint32_t lo = lp_wave_umax((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+            if (best == (((uint64_t)hi << 32) | lo)) {  // one lane: the indices differ
+                out[r] = buf[which];
+                buf[which].y = 0xFFFFFFFFu;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        if (lane < k)
+            buf[lane] = out[lane];
     }
-    for (int j = 64; j < n; ++j) {
-        const uint64_t s = lp_readlane64(b, j - 64);
-        ra += s > a;
-        rb += s > b;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (lane < n && ra < k)
-        buf[ra] = a;
-    if (lane + 64 < n && rb < k)
-        buf[rb] = b;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     st.len = n < k ? n : k;
     if (st.len == k)
-        st.tau = lp_key_score(buf[k - 1]);
+        st.tau = __uint_as_float(__builtin_amdgcn_readfirstlane((int)buf[k - 1].x));
+}
+
+// A score that at least k elements of the tile reach, close to the k-th largest; -inf if fewer are allowed.
+__device__ __forceinline__ float lp_threshold(float lane_max, int k)
+{
+    // the maxima of G lane groups ...
+    float g = lane_max;
+    auto up = [&](uint32_t other) { g = fmaxf(g, __uint_as_float(other)); };
+    int width = 64;  // lanes of a group
+    if (k > 12) {
+        width = 2;
+    } else if (k > 8) {
+        width = 4;
+    } else if (k > 4) {
+        width = 8;
+    } else if (k > 2) {
+        width = 16;
+    }
+    if (k > 2) {
+        up(lp_dpp<0xB1, 0xF>(0, __float_as_uint(g)));
+        if (width >= 4)
+            up(lp_dpp<0x4E, 0xF>(0, __float_as_uint(g)));
+        if (width >= 8)
+            up(lp_dpp<0x141, 0xF>(0, __float_as_uint(g)));
+        if (width >= 16)
+            up(lp_dpp<0x140, 0xF>(0, __float_as_uint(g)));
+        // ... without the smallest G - k of them
+        float thr;
+        if (k * width == 64) {
+            thr = lp_wave_min(g);
+        } else {
+            int above = 0;  // groups with a larger maximum
+            if (width == 2) {
+#pragma unroll
+                for (int i = 0; i < 64; i += 2)
+                    above += __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(g), i)) > g;
+            } else if (width == 4) {
+#pragma unroll
+                for (int i = 0; i < 64; i += 4)
+                    above += __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(g), i)) > g;
+            } else if (width == 8) {
+#pragma unroll
+                for (int i = 0; i < 64; i += 8)
+                    above += __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(g), i)) > g;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 64; i += 16)
+                    above += __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(g), i)) > g;
+            }
+            thr = lp_wave_min(above < k ? g : LP_INF);
+        }
+        if (thr > -LP_INF)
+            return thr;
+    }
+    // k is 1 or 2, or some groups are empty (short rows, few allowed): the k-th largest lane maximum
+    float cur = lane_max, thr;
+    for (int r = 0;; ++r) {
+        thr = lp_wave_max(cur);
+        if (r == k - 1 || thr == -LP_INF)
+            return thr;
+        const int at = __ffsll((unsigned long long)__ballot(cur == thr)) - 1;
+        if (((int)threadIdx.x & 63) == at)
+            cur = -LP_INF;
+    }
+}
+
+// the largest float below v (v finite or -inf, which stays)
+__device__ __forceinline__ float lp_below_value(float v)
+{
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return v == -LP_INF ? v : __uint_as_float(b == 0 ? 0x80000001u : (b >> 31) ? b + 1 : b - 1);
 }
 
 template <int VE>
-__device__ __forceinline__ void lp_collect(const float (&x)[LP_E], float lane_max, float tile_max, int64_t base, int k, int lane, uint64_t *buf, lp_state &st)
+__device__ __forceinline__ void lp_collect(const float (&x)[LP_E], float lane_max, float tile_max, uint32_t base, int rem, int k, int lane, uint2 *buf, lp_state &st)
 {
     constexpr int NV = LP_E / VE;
     const bool full = st.len == k;
     if (full && !(tile_max > st.tau))
         return;  // ties with the last one lose: their indices are higher
-    float thr = st.tau;
-    if (!full) {  // the k-th largest lane maximum
-        float cur = lane_max;
-        for (int r = 0;; ++r) {
-            thr = lp_wave_max(cur);
-            if (r == k - 1 || thr == -LP_INF)
-                break;
-            const uint64_t at = __ballot(cur == thr);
-            if (lane == __ffsll((unsigned long long)at) - 1)
-                cur = -LP_INF;
-        }
-    }
-    int n = st.len, above = 0;
-    uint64_t floor_key = 0;
+    // what is taken: larger scores than the last of a full list, or those from the threshold on
+    const float thr = full ? st.tau : k == 1 ? tile_max : lp_threshold(lane_max, k);
+    const float over = full ? thr : lp_below_value(thr);
+    uint32_t first[NV];  // indices of the lane's vectors
 #pragma unroll
-    for (int e = 0; e < LP_E; ++e) {
-        bool take = x[e] > thr;
-        uint64_t at = __ballot(take);
+    for (int v = 0; v < NV; ++v)
+        first[v] = base + lp_start<VE>(v, lane, rem);
+    int n = st.len;
+    auto gather = [&](int e, float limit) {
+        const bool take = x[e] > limit;
+        const uint64_t at = __ballot(take);
         if (at == 0)
-            continue;
-        above += __popcll(at);
-        if (n + __popcll(at) > LP_BUF) {
-            lp_rank(buf, n, k, lane, st);
-            n = st.len;
-            floor_key = n == k ? buf[k - 1] : 0;
-        }
-        const uint64_t key = lp_key(x[e], (uint32_t)(base + ((e / VE) * 64 + lane) * VE + e % VE));
-        if (floor_key) {
-            take = take && key > floor_key;
-            at = __ballot(take);
-        }
+            return;
         if (take)
-            buf[n + lp_below(at)] = key;
+            buf[n + lp_below(at)] = make_uint2(__float_as_uint(x[e]), first[e / VE] + e % VE);
         n += __popcll(at);
+    };
+#pragma unroll
+    for (int e = 0; e < LP_E / 2; ++e)
+        gather(e, over);
+    if (n <= 64) {
+#pragma unroll
+        for (int e = LP_E / 2; e < LP_E; ++e)
+            gather(e, over);
     }
-    if (!full && thr > -LP_INF && above < k) {  // those equal to the threshold, lowest indices first
-        int need = k - above;
-        for (int v = 0; v < NV && need > 0; ++v) {
-            uint64_t eq[VE];
-            int before = 0, total = 0, own = 0;
+    // Many at once: scores equal to the threshold, of which only the first that are needed may be taken, or rows in rising
+    // order.  Half a tile at a time, ranked in between.
+    if (n > 64) {
+        n = st.len;
+        int above = 0;
+#pragma unroll
+        for (int e = 0; e < LP_E; ++e) {
+            above += __popcll(__ballot(x[e] > thr));
+            gather(e, thr);
+            if (e == LP_E / 2 - 1 && n > 64) {
+                lp_rank<VE == 8>(buf, n, k, lane, st);
+                n = st.len;
+            }
+        }
+        int need = full || !(thr > -LP_INF) ? 0 : k - above;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            int before = 0, total = 0;
 #pragma unroll
             for (int u = 0; u < VE; ++u) {
-                float xe = x[u];  // (x[v * VE + u] without a run-time register index)
-#pragma unroll
-                for (int w = 1; w < NV; ++w)
-                    xe = v == w ? x[w * VE + u] : xe;
-                eq[u] = __ballot(xe == thr);
-                before += lp_below(eq[u]);
-                total += __popcll(eq[u]);
+                const uint64_t at = __ballot(x[v * VE + u] == thr);
+                before += lp_below(at);
+                total += __popcll(at);
             }
+            if (need > 0 && total > 0) {
 #pragma unroll
-            for (int u = 0; u < VE; ++u) {
-                if ((eq[u] >> lane) & 1) {
-                    if (before + own < need)
-                        buf[n + before + own] = lp_key(thr, (uint32_t)(base + (v * 64 + lane) * VE + u));
-                    ++own;
-                }
+                for (int u = 0; u < VE; ++u)
+                    if (x[v * VE + u] == thr) {
+                        if (before < need)
+                            buf[n + before] = make_uint2(__float_as_uint(thr), first[v] + u);
+                        ++before;
+                    }
+                n += total < need ? total : need;
+                need -= total;
             }
-            const int got = total < need ? total : need;
-            n += got;
-            need -= got;
         }
     }
-    lp_rank(buf, n, k, lane, st);
+    lp_rank<VE == 8>(buf, n, k, lane, st);
 }
 
 template <int VE>
-__device__ __forceinline__ void lp_tile(const float (&x)[LP_E], int64_t base, float c2, int k, int lane, uint64_t *buf, lp_state &st)
+__device__ __forceinline__ void lp_tile(const float (&x)[LP_E], uint32_t base, int rem, float c2, int k, int lane, uint2 *buf, lp_state &st)
 {
     float lm = x[0];
 #pragma unroll
@@ -340,7 +495,7 @@ __device__ __forceinline__ void lp_tile(const float (&x)[LP_E], int64_t base, fl
             const float d = (st.m - tm) * c2, f = __builtin_amdgcn_exp2f(d);
             const float w = st.S + (lane == 0 ? (float)st.c : 0.0f);
             st.S = w * f;
-            st.Q = f > 0.0f ? (st.Q + w * d) * f : 0.0f;
+            st.Q = f > 0.0f ? __builtin_fmaf(w, d, st.Q) * f : 0.0f;
         }
         st.m = tm;
         st.c = 0;
@@ -355,19 +510,20 @@ __device__ __forceinline__ void lp_tile(const float (&x)[LP_E], int64_t base, fl
         const float p = less ? __builtin_amdgcn_exp2f(t2) : 0.0f;
         st.c += 64 - __popcll(__ballot(less));
         st.S += p;
-        st.Q += p * fmaxf(t2, -1e30f);  // (0 times -inf)
+        st.Q = __builtin_fmaf(p, fmaxf(t2, -1e30f), st.Q);  // (0 times -inf)
     }
     if (k)
-        lp_collect<VE>(x, lm, tm, base, k, lane, buf, st);
+        lp_collect<VE>(x, lm, tm, base, rem, k, lane, buf, st);
 }
 
-// Joins n <= 64 partial states: lane p < n holds state p and, in LDS, its sorted list of `len` keys at lists + p * LP_KMAX.
-// Results uniform (m, c, S, Q, bad); the k best keys to `out`.  Returns how many there are.
-__device__ __forceinline__ int lp_join(float m, float S, float Q, float c, bool bad, int len, const uint64_t *lists, int k, float c2, int lane, lp_state &st, uint64_t *out)
+// Joins n <= 64 partial states: lane p < n holds state p and its sorted list of `len` at lists + p * LP_KMAX (LDS).
+// Results uniform (m, c, S, Q, bad, len); the k best go to `out`.
+__device__ __forceinline__ void lp_join(float m, float S, float Q, float c, bool bad, int len, const uint2 *lists, int k, float c2, int lane, lp_state &st, uint2 *out)
 {
+    st = lp_state();
     st.bad = __ballot(bad) != 0;
     if (st.bad)
-        return 0;
+        return;
     st.m = lp_wave_max(m);
     const bool has = m > -LP_INF;
     const float d = has ? (m - st.m) * c2 : 0.0f, f = __builtin_amdgcn_exp2f(d);
@@ -376,36 +532,50 @@ __device__ __forceinline__ int lp_join(float m, float S, float Q, float c, bool 
     st.c = (int)lp_wave_sum(top ? c : 0.0f);
     st.S = lp_wave_sum(top ? S : has ? w * f : 0.0f);
     st.Q = lp_wave_sum(top ? Q : has && f > 0.0f ? (Q + w * d) * f : 0.0f);
-    int held = 0, at = 0;
-    uint64_t head = len > 0 ? lists[lane * LP_KMAX] : 0;
-    for (; held < k; ++held) {
+    int at = 0;
+    auto head_of = [&](int i) {
+        const uint2 q = lists[lane * LP_KMAX + i];
+        return lp_key(__uint_as_float(q.x), q.y);
+    };
+    uint64_t head = len > 0 ? head_of(0) : 0;
+    for (; st.len < k; ++st.len) {
         const uint32_t hi = lp_wave_umax((uint32_t)(head >> 32));
         if (hi == 0)
             break;  // (no key of a score has a zero upper word)
         const uint32_t lo = lp_wave_umax((uint32_t)(head >> 32) == hi ? (uint32_t)head : 0u);
         const uint64_t best = ((uint64_t)hi << 32) | lo;
         if (head == best) {  // one lane: the indices differ
-            out[held] = best;
+            out[st.len] = make_uint2(__float_as_uint(lp_key_score(best)), lp_key_index(best));
             ++at;
-            head = at < len ? lists[lane * LP_KMAX + at] : 0;
+            head = at < len ? head_of(at) : 0;
         }
     }
-    return held;
 }
 
+// The kernel's arguments (its first parameter), read when they are needed: those of the last step would otherwise sit in
+// registers, and in spill space, from the start.
+__device__ __forceinline__ const lp_args &lp_late_args()
+{
+    auto *p = (const __attribute__((address_space(4))) lp_args *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const lp_args *)p;
+}
+
+// What is written of rows row0 .. row0 + nrows - 1: lane r holds row r's sums (S and Q of the whole row), its list lies at
+// lists + r * LP_KMAX.
 template <int DT>
-__device__ __forceinline__ void lp_finish(const lp_args &a, int64_t row, const lp_state &st, const uint64_t *buf, int lane)
+__device__ __forceinline__ void lp_finish(int64_t row0, int nrows, float m, float S, float Q, int c, bool bad, int len, const uint2 *lists, int lane)
 {
     using P = lp_type<DT>;
+    const lp_args &a = lp_late_args();
     const float nan = __builtin_nanf("");
-    const float l = st.m > -LP_INF ? log1pf(st.S + (float)(st.c - 1)) : -LP_INF;
-    if (lane == 0) {
-        if (a.stats) {
-            a.stats[2 * row] = st.bad ? nan : st.m;
-            a.stats[2 * row + 1] = st.bad ? nan : l;
-        }
+    const float l = m > -LP_INF ? log1pf(S + (float)(c - 1)) : -LP_INF;
+    if (lane < nrows) {
+        const int64_t row = row0 + lane;
+        if (a.stats)
+            reinterpret_cast<lp_u64 *>(a.stats)[row] = lp_u64{{__float_as_uint(bad ? nan : m), __float_as_uint(bad ? nan : l)}};
         if (a.entropy)
-            a.entropy[row] = st.bad ? nan : st.m > -LP_INF ? l - 0.693147180559945f * (st.Q / (st.S + (float)st.c)) : 0.0f;
+            a.entropy[row] = bad ? nan : m > -LP_INF ? l - 0.693147180559945f * (Q / (S + (float)c)) : 0.0f;
         if (a.logp) {
             float v = 0.0f;
             const int64_t y = a.label64 ? ((const int64_t *)a.labels)[row] : (int64_t)((const int32_t *)a.labels)[row];
@@ -414,88 +584,146 @@ __device__ __forceinline__ void lp_finish(const lp_args &a, int64_t row, const l
                 if (a.err)
                     __hip_atomic_store(a.err, SKM_DEVERR_LABEL, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
             } else if (y >= 0) {
-                if (st.bad) {
+                if (bad) {
                     v = nan;
                 } else if (a.mask && a.mask[row * a.ldmask + y] == 0) {
                     v = -LP_INF;
                 } else {
                     const float s = P::one(((const typename P::T *)a.scores)[row * a.ld + y]);
-                    v = s > -LP_INF ? (s - st.m) * a.inv_t - l : -LP_INF;
+                    v = s > -LP_INF ? (s - m) * a.inv_t - l : -LP_INF;
                 }
             }
             a.logp[row] = v;
         }
     }
-    if (lane < a.k) {
-        const bool there = !st.bad && lane < st.len;
-        const uint64_t key = there ? buf[lane] : 0;
-        if (a.top_index)
-            a.top_index[row * a.k + lane] = there ? (int32_t)lp_key_index(key) : -1;
-        if (a.top_logp)
-            a.top_logp[row * a.k + lane] = there ? (lp_key_score(key) - st.m) * a.inv_t - l : st.bad ? nan : -LP_INF;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int i0 = 0; i0 < nrows * a.k; i0 += 64) {
+        const int i = i0 + lane, r = min(i / max(a.k, 1), nrows - 1), at = i - r * a.k;
+        const float mr = __shfl(m, r), lr = __shfl(l, r);
+        const int lenr = __shfl(len, r);
+        const bool badr = __shfl((int)bad, r) != 0;
+        if (i < nrows * a.k) {
+            const bool there = !badr && at < lenr;
+            const uint2 q = there ? lists[r * LP_KMAX + at] : make_uint2(0, 0xFFFFFFFFu);
+            if (a.top_index)
+                a.top_index[row0 * a.k + i] = (int32_t)q.y;
+            if (a.top_logp)
+                a.top_logp[row0 * a.k + i] = there ? (__uint_as_float(q.x) - mr) * a.inv_t - lr : badr ? nan : -LP_INF;
+        }
     }
 }
 
-// W waves a row (workgroups of max(4, W) waves); SPLIT: a workgroup takes tiles_per_split tiles of a row and leaves its state.
-template <int DT, int MASK, int W, bool SPLIT>
-__global__ __launch_bounds__(W == 16 ? 1024 : 256) void k_log_probabilities(lp_args a)
+// classes of a row from tile t on, at most a tile's; opaque, so that what follows from it is not computed ahead of the loops
+__device__ __forceinline__ int lp_left(int64_t cols, int64_t t)
 {
-    using P = lp_type<DT>;
-    constexpr int NW = W == 16 ? 16 : 4, ROWS = NW / W;
-    __shared__ uint64_t s_buf[NW][LP_BUF];
-    __shared__ uint64_t s_lists[W > 1 ? NW : 1][LP_KMAX];
-    __shared__ float4 s_state[NW];
-    __shared__ int s_len[NW];
+    int rem = (int)min(cols - t * LP_TILE, (int64_t)LP_TILE);
+    rem = __builtin_amdgcn_readfirstlane(rem);
+    asm volatile("" : "+s"(rem));
+    return rem;
+}
+
+// The tiles t0, t0 + step, .. < t1 of one row, each under way while the one before it is worked on.  `next` holds the first
+// one; after the last it holds tile 0 of row `then` (no row: below 0).
+template <int DT, int MASK>
+__device__ __forceinline__ void lp_fetch_tile(const lp_args &a, int64_t row, int64_t t, int lane, lp_raw<DT, MASK> &raw)
+{
+    using T = typename lp_type<DT>::T;
+    lp_fetch<DT, MASK>((const T *)a.scores + row * a.ld + t * LP_TILE, MASK ? a.mask + row * a.ldmask + t * LP_TILE : nullptr,
+                       lp_left(a.cols, t), a.cols, lane, raw);
+}
+template <int DT, int MASK>
+__device__ __forceinline__ void lp_walk(const lp_args &a, int64_t row, int64_t t0, int64_t t1, int step, int64_t then, int lane, uint2 *buf, lp_state &st,
+                                        lp_raw<DT, MASK> &next)
+{
+    for (int64_t t = t0; t < t1; t += step) {
+        float x[LP_E];
+        const int rem = lp_left(a.cols, t);
+        lp_unpack<DT, MASK>(next, rem, lane, x);
+        if (t + step < t1)
+            lp_fetch_tile<DT, MASK>(a, row, t + step, lane, next);
+        else if (then >= 0)
+            lp_fetch_tile<DT, MASK>(a, then, 0, lane, next);
+        if (!st.bad)
+            lp_tile<lp_type<DT>::VE>(x, (uint32_t)(t * LP_TILE), rem, a.c2, a.k, lane, buf, st);
+    }
+    st.S = lp_wave_sum(st.S);
+    st.Q = lp_wave_sum(st.Q);
+}
+
+// A wave a row, `rows_per_wave` <= LP_ROWS rows one after the other.
+constexpr int LP_ROWS = 8;
+template <int DT, int MASK>
+__global__ __launch_bounds__(256, 5) void k_log_probabilities_rows(lp_args a, int rows_per_wave)
+{
+    __shared__ uint2 s_buf[4][LP_BUF];
+    __shared__ uint2 s_lists[4][LP_ROWS * LP_KMAX];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int part = W == 1 ? 0 : wid;
-    const int64_t units = SPLIT ? a.rows * a.nsplit : a.rows;
-    for (int64_t unit0 = (int64_t)blockIdx.x * ROWS; unit0 < units; unit0 += (int64_t)gridDim.x * ROWS) {
-        const int64_t unit = unit0 + (W == 1 ? wid : 0);
-        const int64_t row = SPLIT ? unit / a.nsplit : unit;
-        const int split = SPLIT ? (int)(unit % a.nsplit) : 0;
+    const int64_t tiles = (a.cols + LP_TILE - 1) / LP_TILE;
+    const int64_t row0 = ((int64_t)blockIdx.x * 4 + wid) * rows_per_wave;
+    if (row0 >= a.rows)
+        return;
+    const int nrows = (int)min((int64_t)rows_per_wave, a.rows - row0);
+    float m = 0.0f, S = 0.0f, Q = 0.0f;
+    int c = 0, len = 0;
+    bool bad = false;
+    lp_raw<DT, MASK> next;
+    lp_fetch_tile<DT, MASK>(a, row0, 0, lane, next);
+#pragma unroll 1
+    for (int r = 0; r < nrows; ++r) {
         lp_state st;
-        uint64_t *buf = s_buf[wid];
-        if (unit < units) {
-            const typename P::T *srow = (const typename P::T *)a.scores + row * a.ld;
-            const uint8_t *mrow = MASK ? a.mask + row * a.ldmask : nullptr;
-            const int64_t tiles = (a.cols + LP_TILE - 1) / LP_TILE;
-            const int64_t t0 = SPLIT ? split * a.tiles_per_split : 0, t1 = SPLIT ? min(tiles, t0 + a.tiles_per_split) : tiles;
-            for (int64_t t = t0 + part; t < t1 && !st.bad; t += W) {
-                float x[LP_E];
-                lp_load_tile<DT, MASK>(srow, mrow, t * LP_TILE, a.cols, lane, x);
-                lp_tile<P::VE>(x, t * LP_TILE, a.c2, a.k, lane, buf, st);
-            }
-            st.S = lp_wave_sum(st.S);
-            st.Q = lp_wave_sum(st.Q);
+        lp_walk<DT, MASK>(a, row0 + r, 0, tiles, 1, r + 1 < nrows ? row0 + r + 1 : -1, lane, s_buf[wid], st, next);
+        if (lane < st.len)
+            s_lists[wid][r * LP_KMAX + lane] = s_buf[wid][lane];
+        if (lane == r) {
+            m = st.m;
+            S = st.S;
+            Q = st.Q;
+            c = st.c;
+            len = st.len;
+            bad = st.bad;
         }
-        if (W > 1) {
-            if (lane == 0) {
-                s_state[wid] = make_float4(st.m, st.S, st.Q, st.bad ? -1.0f : (float)st.c);
-                s_len[wid] = st.len;
-            }
-            if (lane < st.len)
-                s_lists[wid][lane] = buf[lane];
-            __syncthreads();
-            if (wid == 0) {
-                const bool own = lane < W;
-                const float4 q = own ? s_state[lane] : make_float4(-LP_INF, 0.0f, 0.0f, 0.0f);
-                st = lp_state();
-                st.len = lp_join(q.x, q.y, q.z, q.w < 0.0f ? 0.0f : q.w, q.w < 0.0f, own ? s_len[lane] : 0, &s_lists[0][0], a.k, a.c2, lane, st, buf);
-            }
-        }
-        if (unit < units && (W == 1 || wid == 0)) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (SPLIT) {
-                if (lane == 0)
-                    a.part[unit] = make_float4(st.m, st.S, st.Q, st.bad ? -1.0f : (float)st.c);
-                if (lane < LP_KMAX)
-                    a.part_keys[unit * LP_KMAX + lane] = lane < st.len ? buf[lane] : 0;
-            } else {
-                lp_finish<DT>(a, row, st, buf, lane);
-            }
-        }
-        if (W > 1)
-            __syncthreads();  // the lists are read before the next row's are written
+    }
+    lp_finish<DT>(row0, nrows, m, S, Q, c, bad, len, s_lists[wid], lane);
+}
+
+// W waves a row; SPLIT: a workgroup takes tiles_per_split tiles of a row and leaves its state.
+template <int DT, int MASK, int W, bool SPLIT>
+__global__ __launch_bounds__(W * 64, W == 4 ? 5 : 4) void k_log_probabilities(lp_args a)
+{
+    __shared__ uint2 s_buf[W][LP_BUF];
+    __shared__ uint2 s_lists[W * LP_KMAX];
+    __shared__ float4 s_state[W];
+    __shared__ int s_len[W];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t unit = blockIdx.x, tiles = (a.cols + LP_TILE - 1) / LP_TILE;
+    const int64_t row = SPLIT ? (uint32_t)unit / (uint32_t)a.nsplit : unit;
+    const int64_t t0 = SPLIT ? (unit - row * a.nsplit) * a.tiles_per_split : 0, t1 = SPLIT ? min(tiles, t0 + a.tiles_per_split) : tiles;
+    lp_state st;
+    uint2 *buf = s_buf[wid];
+    lp_raw<DT, MASK> next;
+    if (t0 + wid < t1)
+        lp_fetch_tile<DT, MASK>(a, row, t0 + wid, lane, next);
+    lp_walk<DT, MASK>(a, row, t0 + wid, t1, W, -1, lane, buf, st, next);
+    if (lane == 0) {
+        s_state[wid] = make_float4(st.m, st.S, st.Q, st.bad ? -1.0f : (float)st.c);
+        s_len[wid] = st.len;
+    }
+    if (lane < st.len)
+        s_lists[wid * LP_KMAX + lane] = buf[lane];
+    __syncthreads();
+    if (wid != 0)
+        return;
+    const bool own = lane < W;
+    const float4 q = own ? s_state[lane] : make_float4(-LP_INF, 0.0f, 0.0f, 0.0f);
+    lp_join(q.x, q.y, q.z, fmaxf(q.w, 0.0f), q.w < 0.0f, own ? s_len[lane] : 0, s_lists, a.k, a.c2, lane, st, buf);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (SPLIT) {
+        if (lane == 0)
+            a.part[unit] = make_float4(st.m, st.S, st.Q, st.bad ? -1.0f : (float)st.c);
+        if (lane < LP_KMAX)
+            a.part_lists[unit * LP_KMAX + lane] = lane < st.len ? buf[lane] : make_uint2(0, 0xFFFFFFFFu);
+    } else {
+        lp_finish<DT>(row, 1, st.m, st.S, st.Q, st.c, st.bad, st.len, buf, lane);
     }
 }
 
@@ -503,27 +731,25 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void k_log_probabilities(lp_a
 template <int DT>
 __global__ __launch_bounds__(64) void k_log_probabilities_join(lp_args a)
 {
-    __shared__ uint64_t s_lists[LP_MAX_SPLITS * LP_KMAX];
-    __shared__ uint64_t s_out[LP_KMAX];
+    __shared__ uint2 s_lists[LP_MAX_SPLITS * LP_KMAX];
+    __shared__ uint2 s_out[LP_KMAX];
     const int lane = threadIdx.x;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const bool own = lane < a.nsplit;
-        const float4 q = own ? a.part[row * a.nsplit + lane] : make_float4(-LP_INF, 0.0f, 0.0f, 0.0f);
-        int len = 0;
-        if (a.k) {
-            for (int i = lane; i < a.nsplit * LP_KMAX; i += 64)
-                s_lists[i] = a.part_keys[row * a.nsplit * LP_KMAX + i];
-            __syncthreads();
-            if (own)
-                for (int i = 0; i < LP_KMAX; ++i)
-                    len += s_lists[lane * LP_KMAX + i] != 0;
-        }
-        lp_state st;
-        st.len = lp_join(q.x, q.y, q.z, q.w < 0.0f ? 0.0f : q.w, q.w < 0.0f, len, s_lists, a.k, a.c2, lane, st, s_out);
+    const int64_t row = blockIdx.x;
+    const bool own = lane < a.nsplit;
+    const float4 q = own ? a.part[row * a.nsplit + lane] : make_float4(-LP_INF, 0.0f, 0.0f, 0.0f);
+    int len = 0;
+    if (a.k) {
+        for (int i = lane; i < a.nsplit * LP_KMAX; i += 64)
+            s_lists[i] = a.part_lists[row * a.nsplit * LP_KMAX + i];
         __syncthreads();
-        lp_finish<DT>(a, row, st, s_out, lane);
-        __syncthreads();
+        if (own)
+            for (int i = 0; i < LP_KMAX; ++i)
+                len += s_lists[lane * LP_KMAX + i].y != 0xFFFFFFFFu;
     }
+    lp_state st;
+    lp_join(q.x, q.y, q.z, fmaxf(q.w, 0.0f), q.w < 0.0f, len, s_lists, a.k, a.c2, lane, st, s_out);
+    __syncthreads();
+    lp_finish<DT>(row, 1, st.m, st.S, st.Q, st.c, st.bad, st.len, s_out, lane);
 }
 
 // ---------------------------------------------------------------------------- gradient
@@ -557,8 +783,13 @@ __global__ __launch_bounds__(256) void k_log_probabilities_grad(lp_grad_args a)
         const int64_t row = unit / tiles, base = (unit - row * tiles) * LP_TILE;
         const T *srow = (const T *)a.scores + row * a.ld;
         T *orow = (T *)a.out + row * a.ldo;
+        const int rem = (int)min(a.cols - base, (int64_t)LP_TILE);
         float x[LP_E];
-        lp_load_tile<DT, MASK>(srow, MASK ? a.mask + row * a.ldmask : nullptr, base, a.cols, lane, x);
+        {  // (in place: what is read of other lanes' elements may be their gradients already, and is dropped)
+            lp_raw<DT, MASK> raw;
+            lp_fetch<DT, MASK>(srow + base, MASK ? a.mask + row * a.ldmask + base : nullptr, rem, a.cols, lane, raw);
+            lp_unpack<DT, MASK>(raw, rem, lane, x);
+        }
         const int64_t y = !a.d_logp ? -1 : a.label64 ? ((const int64_t *)a.labels)[row] : (int64_t)((const int32_t *)a.labels)[row];
         const bool wrong = y < -1 || y >= a.cols;
         if (wrong && a.err && lane == 0)
@@ -581,52 +812,51 @@ __global__ __launch_bounds__(256) void k_log_probabilities_grad(lp_grad_args a)
             const float s = P::one(srow[y]);
             const bool allowed = s != -LP_INF && (!MASK || a.mask[row * a.ldmask + y] != 0);
             const float z = (s - m) * a.inv_t - l;
-            const float v = allowed ? -gi * expm1f(z) - __builtin_amdgcn_exp2f(z * 1.44269504088896f) * hi * (fmaxf((s - m) * a.inv_t, -1e30f) + hl) : 0.0f;
+            const float d = allowed ? -gi * expm1f(z) - __builtin_amdgcn_exp2f(z * 1.44269504088896f) * hi * (fmaxf((s - m) * a.inv_t, -1e30f) + hl) : 0.0f;
 #pragma unroll
             for (int e = 0; e < LP_E; ++e)
-                if ((int)((off / VE) / 64) == e / VE && (int)(off % VE) == e % VE)
-                    x[e] = v;
+                if ((int)off / VE / 64 == e / VE && (int)off - lp_start<VE>(e / VE, lane, rem) == e % VE)
+                    x[e] = d;
         }
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int64_t at = base + (v * 64 + lane) * VE;
-            if (at + VE <= a.cols) {
-                lp_u128 raw;
-                T o[VE];
+            const int at = lp_start<VE>(v, lane, rem), drop = (v * 64 + lane) * VE - at;
+            T o[VE];
 #pragma unroll
-                for (int u = 0; u < VE; ++u)
-                    o[u] = P::round(x[v * VE + u]);
+            for (int u = 0; u < VE; ++u)
+                o[u] = P::round(x[v * VE + u]);
+            if (drop == 0) {
+                lp_u128 raw;
                 __builtin_memcpy(&raw, o, 16);
-                *reinterpret_cast<lp_u128 *>(orow + at) = raw;
+                *reinterpret_cast<lp_u128 *>(orow + base + at) = raw;
             } else {
 #pragma unroll
                 for (int u = 0; u < VE; ++u)
-                    if (at + u < a.cols)
-                        orow[at + u] = P::round(x[v * VE + u]);
+                    if (u >= drop)
+                        orow[base + at + u] = o[u];
             }
         }
     }
 }
 
-// How a row is cut.  A wave's tile costs about as much as a wave's join, so rows are only cut where whole rows would not
-// keep the chip's waves busy.
+// How a row is cut: a wave a row where that fills the chip, else several waves of a workgroup, else several workgroups.
 struct lp_cut {
-    int waves, nsplit;
+    int waves, rows_per_wave, nsplit;
     int64_t tiles_per_split;
 };
 
 lp_cut lp_plan(const skm_ctx *ctx, int64_t rows, int64_t cols)
 {
-    const int64_t tiles = skm_ceil_div(cols, LP_TILE), want = (int64_t)ctx->usable_cus * 8;
-    lp_cut c = {1, 1, tiles};
-    if (tiles == 1 || rows >= want)
+    const int64_t tiles = skm_ceil_div(cols, LP_TILE), cus = ctx->usable_cus, want = cus * 16;  // waves
+    lp_cut c = {1, 1, 1, tiles};
+    if (tiles == 1 || rows >= want / 2) {
+        c.rows_per_wave = (int)std::min<int64_t>(LP_ROWS, std::max<int64_t>(1, rows / (want * 2)));
         return c;
-    c.waves = tiles <= 4 || rows * 4 >= want ? 4 : 16;
-    const int64_t per_wave = 2;  // tiles, at least
-    if (c.waves == 16 && rows * 16 < want && tiles > 16 * per_wave) {
-        int64_t s = skm_ceil_div(want, rows * 16);
-        s = std::min<int64_t>(s, tiles / (16 * per_wave));
-        s = std::min<int64_t>(s, LP_MAX_SPLITS);
+    }
+    // one workgroup a row: four waves, or sixteen where they have no more than four tiles each
+    c.waves = tiles <= 8 || tiles > 64 || rows * 4 >= want ? 4 : 16;
+    if (tiles > 64) {  // several a row: what the compute units hold at once (four workgroups each), two tiles a wave at least
+        const int64_t s = std::min<int64_t>(std::min<int64_t>(4 * cus / rows, tiles / 8), LP_MAX_SPLITS);
         if (s > 1) {
             c.tiles_per_split = skm_ceil_div(tiles, s);
             c.nsplit = (int)skm_ceil_div(tiles, c.tiles_per_split);
@@ -635,26 +865,47 @@ lp_cut lp_plan(const skm_ctx *ctx, int64_t rows, int64_t cols)
     return c;
 }
 
-template <int DT, int MASK>
-int lp_launch(skm_ctx *ctx, const lp_args &a, const lp_cut &cut)
+// `rows` rows from row0 on: a launch holds at most 2^32 work-items
+lp_args lp_rows_from(const lp_args &whole, int64_t row0, int64_t rows, int64_t elem)
 {
-    const int64_t most = (int64_t)1 << 30;
-    if (cut.nsplit > 1) {
-        k_log_probabilities<DT, MASK, 16, true><<<(unsigned)std::min(most, a.rows * cut.nsplit), 1024, 0, ctx->stream>>>(a);
-        SKM_TRY(skm_check_launch("k_log_probabilities"));
-        k_log_probabilities_join<DT><<<(unsigned)std::min(most, a.rows), 64, 0, ctx->stream>>>(a);
-        return skm_check_launch("k_log_probabilities_join");
-    }
-    if (cut.waves == 1)
-        k_log_probabilities<DT, MASK, 1, false><<<(unsigned)std::min(most, skm_ceil_div(a.rows, 4)), 256, 0, ctx->stream>>>(a);
-    else if (cut.waves == 4)
-        k_log_probabilities<DT, MASK, 4, false><<<(unsigned)std::min(most, a.rows), 256, 0, ctx->stream>>>(a);
-    else
-        k_log_probabilities<DT, MASK, 16, false><<<(unsigned)std::min(most, a.rows), 1024, 0, ctx->stream>>>(a);
-    return skm_check_launch("k_log_probabilities");
+    lp_args a = whole;
+    a.rows = rows;
+    a.scores = (const uint8_t *)whole.scores + row0 * whole.ld * elem;
+    a.mask = whole.mask ? whole.mask + row0 * whole.ldmask : nullptr;
+    a.labels = whole.labels ? (const uint8_t *)whole.labels + row0 * (whole.label64 ? 8 : 4) : nullptr;
+    a.logp = whole.logp ? whole.logp + row0 : nullptr;
+    a.entropy = whole.entropy ? whole.entropy + row0 : nullptr;
+    a.stats = whole.stats ? whole.stats + 2 * row0 : nullptr;
+    a.top_index = whole.top_index ? whole.top_index + row0 * whole.k : nullptr;
+    a.top_logp = whole.top_logp ? whole.top_logp + row0 * whole.k : nullptr;
+    return a;
 }
 
-// what both entry points check; sets *elem to the bytes of a score
+template <int DT, int MASK>
+int lp_launch(skm_ctx *ctx, const lp_args &whole, const lp_cut &cut)
+{
+    constexpr int64_t MOST = (int64_t)1 << 21;  // workgroups
+    if (cut.nsplit > 1) {                       // (only where rows are few)
+        k_log_probabilities<DT, MASK, 4, true><<<(unsigned)(whole.rows * cut.nsplit), 256, 0, ctx->stream>>>(whole);
+        SKM_TRY(skm_check_launch("k_log_probabilities"));
+        k_log_probabilities_join<DT><<<(unsigned)whole.rows, 64, 0, ctx->stream>>>(whole);
+        return skm_check_launch("k_log_probabilities_join");
+    }
+    const int64_t step = cut.waves == 1 ? MOST * 4 * cut.rows_per_wave : MOST;
+    for (int64_t row0 = 0; row0 < whole.rows; row0 += step) {
+        const lp_args a = lp_rows_from(whole, row0, std::min(step, whole.rows - row0), sizeof(typename lp_type<DT>::T));
+        if (cut.waves == 1)
+            k_log_probabilities_rows<DT, MASK><<<(unsigned)skm_ceil_div(a.rows, 4 * cut.rows_per_wave), 256, 0, ctx->stream>>>(a, cut.rows_per_wave);
+        else if (cut.waves == 4)
+            k_log_probabilities<DT, MASK, 4, false><<<(unsigned)a.rows, 256, 0, ctx->stream>>>(a);
+        else
+            k_log_probabilities<DT, MASK, 16, false><<<(unsigned)a.rows, 1024, 0, ctx->stream>>>(a);
+        SKM_TRY(skm_check_launch("k_log_probabilities"));
+    }
+    return SKM_OK;
+}
+
+// what both entry points check
 int lp_check(const char *who, skm_ctx *ctx, int dtype, int64_t rows, int64_t cols, const void *d_scores, int64_t ld, const uint8_t *d_mask, int64_t ldmask,
              int label_bits, double temperature)
 {
@@ -711,9 +962,9 @@ extern "C" int skm_log_probabilities(skm_ctx *ctx, int dtype, int64_t rows, int6
     if (cut.nsplit > 1) {
         void *p;
         const size_t units = (size_t)rows * (size_t)cut.nsplit;
-        SKM_TRY(skm_ws(ctx, WS_A, units * (sizeof(float4) + LP_KMAX * sizeof(uint64_t)), &p));
+        SKM_TRY(skm_ws(ctx, WS_A, units * (sizeof(float4) + LP_KMAX * sizeof(uint2)), &p));
         a.part = (float4 *)p;
-        a.part_keys = (uint64_t *)((uint8_t *)p + units * sizeof(float4));
+        a.part_lists = (uint2 *)((uint8_t *)p + units * sizeof(float4));
     }
     SKM_PROF(ctx, "k_log_probabilities");
     switch (dtype * 2 + (d_mask ? 1 : 0)) {
@@ -768,7 +1019,7 @@ extern "C" int skm_log_probabilities_backward(skm_ctx *ctx, int dtype, int64_t r
     a.ldo = ldg;
     a.err = ctx->d_err;
     const int64_t units = rows * skm_ceil_div(cols, LP_TILE);
-    const unsigned grid = (unsigned)std::min<int64_t>((int64_t)1 << 30, skm_ceil_div(units, 4));
+    const unsigned grid = (unsigned)std::min<int64_t>((int64_t)1 << 23, skm_ceil_div(units, 4));
     SKM_PROF(ctx, "k_log_probabilities_grad");
 #define LP_GRAD(DT, MASK) k_log_probabilities_grad<DT, MASK><<<grid, 256, 0, ctx->stream>>>(a)
     switch (dtype * 2 + (d_mask ? 1 : 0)) {
