@@ -374,6 +374,9 @@ def is_device_array(x) -> bool:
     return isinstance(x, DeviceArray) or hasattr(type(x), "__cuda_array_interface__")
 
 
+_TENSOR_TYPES = {}  # type string by dtype object, of arrays that also answer data_ptr() / stride() (see array_view)
+
+
 def array_view(ctx: "Context", x, name: str, ndim: int, types, writable: bool = False):
     """(pointer, shape, row stride in elements, type string) of a device array of this library or of another one
     (`__cuda_array_interface__`), as the entry points take them: the elements of a row next to each other, rows that do not
@@ -385,24 +388,17 @@ def array_view(ctx: "Context", x, name: str, ndim: int, types, writable: bool = 
         if typestr == "|V2":
             typestr = "<V2"
     else:
-        iface = getattr(x, "__cuda_array_interface__", None)
-        if iface is None:
-            raise TypeError(f"{name}: want an array on the device (a DeviceArray or an object with __cuda_array_interface__), got {type(x).__name__}")
-        shape, typestr, (ptr, readonly), strides = iface["shape"], iface["typestr"], iface["data"], iface.get("strides")
-        if iface.get("mask") is not None:
-            raise ValueError(f"{name}: masked arrays are not taken")
-        if writable and readonly:
-            raise ValueError(f"{name}: the array is read-only")
-        where = getattr(x, "device", None)
-        device = getattr(where, "index", None)
-        if not isinstance(device, int):
-            device = getattr(where, "id", None)
-        if not isinstance(device, int):
-            device = ctx.device
-            if ptr:
-                out = C.c_int(-1)
-                _check(ctx.lib, ctx.lib.skm_pointer_device(_p(ptr), C.byref(out)))
-                device = out.value
+        # Tensors whose dtype has come through the interface before answer its questions one by one in half a microsecond;
+        # building the interface's dictionary takes them two, and a call passes up to seven arrays.
+        try:
+            typestr = _TENSOR_TYPES[x.dtype]
+            fast = x.is_cuda and not x.requires_grad
+        except (AttributeError, KeyError, TypeError):
+            fast = False
+        if fast:
+            ptr, shape, strides, device = x.data_ptr(), x.shape, x.stride(), x.device.index
+        else:
+            ptr, shape, strides, device, typestr = _from_interface(ctx, x, name, writable)
     if typestr not in types:
         raise TypeError(f"{name}: elements of type {typestr}, want one of {', '.join(types)}")
     if device != ctx.device:
@@ -412,14 +408,42 @@ def array_view(ctx: "Context", x, name: str, ndim: int, types, writable: bool = 
     cols = shape[-1]
     ld = cols
     if strides is not None:
-        size = _ITEMSIZE[typestr]
-        if cols > 1 and strides[-1] != size:
+        if cols > 1 and strides[-1] != 1:
             raise ValueError(f"{name}: the elements of a row must lie next to each other")
         if ndim == 2 and shape[0] > 1:
-            ld, rest = divmod(strides[0], size)
-            if rest or ld < cols:
+            ld = strides[0]
+            if ld < cols or ld != int(ld):
                 raise ValueError(f"{name}: rows that overlap, run backwards or start between elements")
+            ld = int(ld)
     return ptr, shape, ld, typestr
+
+
+def _from_interface(ctx: "Context", x, name: str, writable: bool):
+    """(pointer, shape, strides in elements or None, device, type string) by `__cuda_array_interface__`."""
+    iface = getattr(x, "__cuda_array_interface__", None)
+    if iface is None:
+        raise TypeError(f"{name}: want an array on the device (a DeviceArray or an object with __cuda_array_interface__), got {type(x).__name__}")
+    shape, typestr, (ptr, readonly), strides = tuple(iface["shape"]), iface["typestr"], iface["data"], iface.get("strides")
+    if iface.get("mask") is not None:
+        raise ValueError(f"{name}: masked arrays are not taken")
+    if writable and readonly:
+        raise ValueError(f"{name}: the array is read-only")
+    where = getattr(x, "device", None)
+    device = getattr(where, "index", None)
+    if not isinstance(device, int):
+        device = getattr(where, "id", None)
+    if not isinstance(device, int):
+        device = ctx.device
+        if ptr:
+            out = C.c_int(-1)
+            _check(ctx.lib, ctx.lib.skm_pointer_device(_p(ptr), C.byref(out)))
+            device = out.value
+    if strides is not None:
+        size = _ITEMSIZE.get(typestr, 1)
+        strides = tuple(s // size if s % size == 0 else s / size for s in strides)
+    if typestr in _ITEMSIZE and all(hasattr(x, a) for a in ("data_ptr", "stride", "is_cuda", "requires_grad", "dtype")):
+        _TENSOR_TYPES[x.dtype] = typestr
+    return ptr, shape, strides, device, typestr
 
 
 class Context:

@@ -512,6 +512,131 @@ __global__ __launch_bounds__(256, (BM + BN) > 256 ? 1 : 2) void k_linear(ln_gemm
     ln_store_tile<DT, FM, FN, SPLIT>(g, at, acc, reinterpret_cast<float *>(s_t), wid, wr * TM, wc * TN, lane);
 }
 
+// ---- few rows: the weights are read once, and that is the time
+// A workgroup computes 16 columns of up to 16 MB rows: its NW waves share the contraction in 128-byte lines, both operands
+// come straight from memory into the matrix operands (16 x 16 products; 16 bytes a lane, rows of any alignment), and the
+// waves' sums are added up in LDS in order.  One launch and no scratch: what a single query costs is a launch and the
+// weights' way through memory.
+template <int DT>
+struct ln_small;
+template <>
+struct ln_small<0> {
+    static __device__ __forceinline__ f32x4 mfma(f32x4 a, f32x4 b, f32x4 c)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // (lane quarter h holds columns 4 h .. 4 h + 3: the i-th product takes columns 4 h + i)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+template <>
+struct ln_small<1> {
+    static __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct ln_small<2> {
+    static __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+template <int DT, int MB, int NW>
+__global__ __launch_bounds__(NW * 64) void k_linear_few(ln_gemm g)
+{
+    using P = ln_type<DT>;
+    using T = typename P::T;
+    using V = typename P::V;
+    constexpr int VE = P::VE, LINE = 128 / (int)sizeof(T), HALVES = LINE / (4 * VE);
+    static_assert(HALVES == 2, "a line is two steps of four 16-byte pieces");
+    constexpr int AHEAD = MB == 1 ? 4 : 2;  // lines whose loads are under way together
+    __shared__ f32x4 s_sum[NW][MB][64];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, piece = lane >> 4;
+    const int64_t col0 = (int64_t)blockIdx.x * 16;
+    const T *const w = reinterpret_cast<const T *>(g.b + min(col0 + r, g.n - 1) * g.ldb);  // (rows past the end: any, not stored)
+    const T *x[MB];
+#pragma unroll
+    for (int q = 0; q < MB; ++q)
+        x[q] = reinterpret_cast<const T *>(g.a + min((int64_t)q * 16 + r, g.m - 1) * g.lda);
+    f32x4 acc[MB];
+#pragma unroll
+    for (int q = 0; q < MB; ++q)
+        acc[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // 16 bytes of a row from column c on, zeros behind the contraction's end: a piece that would reach past it starts earlier, at
+    // the last whole one, and what that repeats is dropped (from both operands alike: which lane holds a column is all one)
+    auto read = [&](const T *row, int64_t c) {
+        V v;
+        if (g.k >= VE) {
+            const int64_t start = min(c, g.k - VE), drop = c - start;
+            const ln_u128 raw = *reinterpret_cast<const ln_u128 *>(row + start);
+            __builtin_memcpy(&v, &raw, 16);
+#pragma unroll
+            for (int u = 0; u < VE; ++u)
+                v[u] = u < drop ? (T)0.0f : v[u];
+        } else {
+#pragma unroll
+            for (int u = 0; u < VE; ++u)
+                v[u] = c + u < g.k ? row[c + u] : (T)0.0f;
+        }
+        return v;
+    };
+    const int64_t lines = (g.k + LINE - 1) / LINE, whole = g.k / LINE;
+    int64_t l = wid;
+    for (; l + (AHEAD - 1) * NW < whole; l += AHEAD * NW) {
+        V vw[AHEAD][2], vx[AHEAD][2][MB];
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int64_t c = (l + d * NW) * LINE + (h * 4 + piece) * VE;
+                ln_u128 raw = *reinterpret_cast<const ln_u128 *>(w + c);
+                __builtin_memcpy(&vw[d][h], &raw, 16);
+#pragma unroll
+                for (int q = 0; q < MB; ++q) {
+                    raw = *reinterpret_cast<const ln_u128 *>(x[q] + c);
+                    __builtin_memcpy(&vx[d][h][q], &raw, 16);
+                }
+            }
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < MB; ++q)
+                    acc[q] = ln_small<DT>::mfma(vw[d][h], vx[d][h][q], acc[q]);
+    }
+    for (; l < lines; l += NW)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t c = l * LINE + (h * 4 + piece) * VE;
+            const V vw = read(w, c);
+#pragma unroll
+            for (int q = 0; q < MB; ++q)
+                acc[q] = ln_small<DT>::mfma(vw, read(x[q], c), acc[q]);
+        }
+#pragma unroll
+    for (int q = 0; q < MB; ++q)
+        s_sum[wid][q][lane] = acc[q];
+    __syncthreads();
+    // cell (row 16 q + r, column 4 piece + u) of the tile is register u of lane (piece, r)
+    for (int t = threadIdx.x; t < MB * 256; t += NW * 64) {
+        const int q = t >> 8, row = (t >> 4) & 15, col = t & 15;
+        const int64_t i = q * 16 + row, j = col0 + col;
+        if (i >= g.m || j >= g.n)
+            continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int s = 0; s < NW; ++s)
+            v += reinterpret_cast<const float *>(&s_sum[s][q][(col >> 2) * 16 + row])[col & 3];
+        if (g.bias)
+            v += (float)((const T *)g.bias)[j];
+        if (g.preact)
+            ((T *)g.preact)[i * g.ldp + j] = (T)v;
+        v = ln_act(g.act, v);
+        if (g.residual)
+            v += (float)((const T *)g.residual)[i * g.ldr + j];
+        ((T *)g.out)[i * g.ldo + j] = (T)v;
+    }
+}
+
 // the sums over the splits, in order, and the epilogue
 template <int DT>
 __global__ __launch_bounds__(256) void k_linear_join(ln_gemm g)
@@ -798,6 +923,33 @@ int gemm(skm_ctx *ctx, ln_gemm g)
     return SKM_OK;
 }
 
+// Few rows read the weights straight from memory.  Measured, microseconds, 1 / 16 / 32 rows of k = 4096, n = 1000, bfloat16: 6.8 / 9.0 /
+// 12.9 against 11.2 / 13.2 / 13.2 by tiles; k = 16384, n = 4096: 26 / 32 / 44 against 30 / 30 / 31; k = 300, 64 rows: 6.8 against 12.7.
+bool few_rows(int64_t m, int64_t kbytes) { return m <= 16 || (m <= 64 && kbytes <= 1024); }
+
+template <int DT, int MB>
+int launch_few(skm_ctx *ctx, const ln_gemm &g)
+{
+    const int64_t groups = skm_ceil_div(g.n, 16);
+    SKM_REQUIRE(groups < ((int64_t)1 << 22), SKM_E_OVERFLOW, "skm_linear: too many columns");
+    SKM_PROF(ctx, "k_linear_few");
+    if (g.k * (int64_t)elem_bytes(DT) >= 4096)
+        k_linear_few<DT, MB, 16><<<(unsigned)groups, 1024, 0, ctx->stream>>>(g);
+    else
+        k_linear_few<DT, MB, 4><<<(unsigned)groups, 256, 0, ctx->stream>>>(g);
+    return skm_check_launch("k_linear_few");
+}
+
+template <int DT>
+int launch_few(skm_ctx *ctx, const ln_gemm &g)
+{
+    if (g.m <= 16)
+        return launch_few<DT, 1>(ctx, g);
+    if (g.m <= 32)
+        return launch_few<DT, 2>(ctx, g);
+    return launch_few<DT, 4>(ctx, g);
+}
+
 // The operand as the product reads it: where it lies if its rows start on 16-byte boundaries and hold whole 16-byte
 // pieces, else a padded copy in scratch.
 template <int DT>
@@ -844,8 +996,6 @@ int forward(skm_ctx *ctx, int act, int64_t m, int64_t n, int64_t k, const void *
     g.m = m;
     g.n = n;
     g.k = k;
-    SKM_TRY(ready<DT>(ctx, WS_A, m, k, x, ldx, &g.a, &g.lda));
-    SKM_TRY(ready<DT>(ctx, WS_B, n, k, w, ldw, &g.b, &g.ldb));
     g.act = act;
     g.bias = bias;
     g.residual = residual;
@@ -854,6 +1004,16 @@ int forward(skm_ctx *ctx, int act, int64_t m, int64_t n, int64_t k, const void *
     g.ldp = ldp;
     g.out = y;
     g.ldo = ldy;
+    if (few_rows(m, k * (int64_t)elem_bytes(DT))) {
+        constexpr int64_t es = (int64_t)elem_bytes(DT);
+        g.a = (const uint8_t *)x;
+        g.lda = ldx * es;
+        g.b = (const uint8_t *)w;
+        g.ldb = ldw * es;
+        return launch_few<DT>(ctx, g);
+    }
+    SKM_TRY(ready<DT>(ctx, WS_A, m, k, x, ldx, &g.a, &g.lda));
+    SKM_TRY(ready<DT>(ctx, WS_B, n, k, w, ldw, &g.b, &g.ldb));
     return gemm<DT>(ctx, g);
 }
 

@@ -597,7 +597,7 @@ def _activation(name) -> int:
 
 
 def _expect(name: str, shape, want) -> None:
-    if tuple(shape) != tuple(want):
+    if shape != want:
         raise ValueError(f"{name}: shape {tuple(shape)}, want {tuple(want)}")
 
 
