@@ -92,7 +92,8 @@ __device__ __forceinline__ float ln_slope(int act, float z)
         return 0.5f * (1.0f + erff(z * 0.707106781186547524f)) + z * __expf(-0.5f * z * z) * 0.398942280401432678f;
     case ACT_GELU_TANH: {
         const float u2 = 1.59576912160573071f * (z + 0.044715f * z * z * z), s = ln_sigmoid(u2);
-        return s + z * s * (1.0f - s) * 1.59576912160573071f * (1.0f + 0.134145f * z * z);
+        const float bell = s * (1.0f - s);  // (0 from |z| = 10 on, where z z may be infinite)
+        return bell == 0.0f ? s : s + z * bell * 1.59576912160573071f * (1.0f + 0.134145f * z * z);
     }
     case ACT_SILU: {
         const float s = ln_sigmoid(z);
@@ -993,13 +994,13 @@ int gemm(skm_ctx *ctx, ln_gemm g)
 
 // Few rows read the weights straight from memory.  Measured, microseconds, 1 / 16 / 32 rows of k = 4096, n = 1000, bfloat16: 6.8 / 9.0 /
 // 12.9 against 11.2 / 13.2 / 13.2 by tiles; k = 16384, n = 4096: 26 / 32 / 44 against 30 / 30 / 31; k = 300, 64 rows: 6.8 against 12.7.
-bool few_rows(int64_t m, int64_t kbytes) { return m <= 16 || (m <= 64 && kbytes <= 1024); }
+// (A launch holds less than 2^32 threads: 2^25 columns are 2^21 workgroups of up to 2^10.)
+bool few_rows(int64_t m, int64_t n, int64_t kbytes) { return (m <= 16 || (m <= 64 && kbytes <= 1024)) && n <= (int64_t)1 << 25; }
 
 template <int DT, int MB>
 int launch_few(skm_ctx *ctx, const ln_gemm &g)
 {
     const int64_t groups = skm_ceil_div(g.n, 16);
-    SKM_REQUIRE(groups < ((int64_t)1 << 22), SKM_E_OVERFLOW, "skm_linear: too many columns");
     SKM_PROF(ctx, "k_linear_few");
     if (g.k * (int64_t)elem_bytes(DT) >= 4096)
         k_linear_few<DT, MB, 16><<<(unsigned)groups, 1024, 0, ctx->stream>>>(g);
@@ -1062,7 +1063,7 @@ int forward(skm_ctx *ctx, int act, int64_t m, int64_t n, int64_t k, const void *
     g.ldp = ldp;
     g.out = y;
     g.ldo = ldy;
-    if (few_rows(m, k * (int64_t)elem_bytes(DT))) {
+    if (few_rows(m, n, k * (int64_t)elem_bytes(DT))) {
         constexpr int64_t es = (int64_t)elem_bytes(DT);
         g.a = (const uint8_t *)x;
         g.lda = ldx * es;

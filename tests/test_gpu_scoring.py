@@ -550,6 +550,83 @@ def test_matrices_of_any_stride_and_alignment(ctx, dt, pad, lead):
         assert (flat[:lead] == 77.0).all() and (flat[lead:].reshape(rows, cols + pad)[:, cols:] == 77.0).all()
 
 
+# outputs m x n, contraction k: together they take every tile, whole contractions and contractions in parts, for both widths of types
+TILES = [(70, 74, 72), (70, 74, 2056), (8200, 72, 74), (2050, 1032, 130), (70, 2056, 4102), (1030, 4102, 72), (8200, 72, 4106), (2050, 2054, 522), (4096, 2048, 2080), (4094, 4096, 1034)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m, n, k", TILES)
+def test_every_tile_in_every_orientation(ctx, m, n, k, dt):
+    """One product three times: forward, as a gradient of inputs (b across the contraction) and as a gradient of weights (both across)."""
+    a, b = whole_numbers((m, k), 1, 2), whole_numbers((n, k), 2, 2)
+    want = as_type(a @ b.T, dt)  # (sums below 2^24: exact in float32)
+    da, db, dat, dbt = (ctx.to_device(rounded(v, dt)[0]) for v in (a, b, a.T, b.T))
+    assert np.array_equal(values(engine.linear(ctx, da, db).download(), dt), want)
+    dx, _, _ = engine.linear_backward(ctx, da, None, dbt, dw=None, dbias=None)
+    assert np.array_equal(values(dx.download(), dt), want)
+    _, dw, dbias = engine.linear_backward(ctx, dat, dbt, None, dx=None)
+    assert np.array_equal(values(dw.download(), dt), want)
+    assert np.array_equal(values(dbias.download(), dt), as_type(a.sum(axis=1, dtype=np.float64), dt))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_rows_that_lie_megabytes_apart(ctx, dt):
+    """Rows 2^24 bytes apart and more, 300 of them: offsets inside a tile pass 32 bits.  Written and read back by products with the identity."""
+    m, n, k = 300, 72, 88
+    size = np.dtype(TYPES[dt]).itemsize
+    ld = (1 << 24) // size + 8
+    x, w, eye = whole_numbers((m, k), 1), whole_numbers((n, k), 2), np.eye(k, dtype=np.float32)
+    g = whole_numbers((m, n), 3)
+    dx, dw, dg, deye, deyen = (ctx.to_device(rounded(v, dt)[0]) for v in (x, w, g, eye, np.eye(n, dtype=np.float32)))
+    far = ctx.empty(m * ld, TYPES[dt])
+    xf, yf, gf = (Strided(far, (m, c), ld, lead) for c, lead in ((k, 0), (n, 4096), (n, 8192)))
+    engine.linear(ctx, dx, deye, out=xf)
+    engine.linear(ctx, dg, deyen, out=gf)
+    engine.linear(ctx, xf, dw, residual=gf, out=yf)
+    want = x @ w.T + g
+    assert np.array_equal(values(engine.linear(ctx, yf, deyen).download(), dt), as_type(want, dt))
+    gx, gw, gb = engine.linear_backward(ctx, gf, xf, dw)
+    assert np.array_equal(values(gx.download(), dt), as_type(g @ w, dt))
+    assert np.array_equal(values(gw.download(), dt), as_type(g.T @ x, dt))
+    assert np.array_equal(values(gb.download(), dt), as_type(g.sum(axis=0), dt))
+    # weights that far apart: few rows, many rows, and across the contraction
+    engine.linear(ctx, dw, deye, out=Strided(far, (n, k), ld))
+    wf = Strided(far, (n, k), ld)
+    assert np.array_equal(values(engine.linear(ctx, dx, wf).download(), dt), as_type(x @ w.T, dt))
+    few = ctx.to_device(rounded(x[:3], dt)[0])
+    assert np.array_equal(values(engine.linear(ctx, few, wf).download(), dt), as_type(x[:3] @ w.T, dt))
+    gx, _, _ = engine.linear_backward(ctx, dg, None, wf, dw=None, dbias=None)
+    assert np.array_equal(values(gx.download(), dt), as_type(g @ w, dt))
+
+
+def test_more_than_two_to_the_31_outputs(ctx):
+    """66000 x 33000 outputs, looked at by columns and rows at the ends (a product with the identity copies them out)."""
+    m, n, k = 66000, 33000, 8
+    x, w = whole_numbers((m, k), 1), whole_numbers((n, k), 2)
+    y = engine.linear(ctx, ctx.to_device(rounded(x, "bf16")[0]), ctx.to_device(rounded(w, "bf16")[0]))
+    eye = ctx.to_device(rounded(np.eye(64, dtype=np.float32), "bf16")[0])
+    for i, j in ((0, 0), (m - 5, 0), (0, n - 64), (m - 5, n - 64), (65100, 32768)):
+        block = engine.linear(ctx, Strided(y, (5, 64), n, i * n + j), eye)
+        assert np.array_equal(values(block.download(), "bf16"), as_type(x[i:i + 5] @ w[j:j + 64].T, "bf16"))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("name", ["none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid"])
+def test_slopes_far_from_zero(ctx, name, dt):
+    """Past |z| = 2^7 every activation is a constant or the identity to float32: slopes of 0 or 1, also where z z is past the type's largest value."""
+    z = np.array([[200.0], [-200.0], [1e10], [-1e10], [1e20], [-1e20], [2.0 ** 126], [-2.0 ** 126]], np.float32)
+    one = rounded(np.ones((1, 1), np.float32), dt)[0]
+    _, _, db = engine.linear_backward(ctx, *(ctx.to_device(v) for v in (rounded(np.ones((1, 8), np.float32), dt)[0],)), None, None, activation=name,
+                                      preact=ctx.to_device(rounded(z.reshape(1, 8), dt)[0]), dx=None, dw=None)
+    up = {"none": 1.0, "sigmoid": 0.0}.get(name, 1.0)
+    down = 1.0 if name == "none" else 0.0
+    assert np.array_equal(values(db.download(), dt), np.tile([up, down], 4))
+    y = engine.linear(ctx, ctx.to_device(rounded(z, dt)[0]), ctx.to_device(one), activation=name).download()
+    zt = rounded(z, dt)[1][:, 0]
+    want = {"none": zt, "sigmoid": (zt > 0).astype(float)}.get(name, np.maximum(zt, 0))
+    assert np.array_equal(values(y, dt)[:, 0], want)
+
+
 def test_infinities_and_nan_stay_in_their_rows(ctx):
     x, w = whole_numbers((40, 90), 1), whole_numbers((50, 90), 2)
     w[w == 0] = 1
