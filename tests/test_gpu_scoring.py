@@ -335,6 +335,31 @@ def gradient_bound(want, s, labels, gl, gh, T, cols, dt):
     return b / T
 
 
+def test_more_rows_than_one_launch_holds(ctx):
+    """2^26 and some rows of two classes: a launch takes 2^26 of them.  Rows repeat with a period that no power of two divides."""
+    n, period = (1 << 26) + 37, 1009
+    rng = np.random.default_rng(6)
+    w, s = rounded(rng.normal(size=(period, 2)), "bf16")
+    labels = rng.integers(0, 2, period)
+    times = n // period + 1
+    out = apply.log_probabilities(ctx, ctx.to_device(np.tile(w, (times, 1))[:n]), ctx.to_device(np.tile(labels.astype(np.int32), times)[:n]), k=0)
+    logp = out.logp.download()
+    want = plain_logp(s, labels, 1, 1.0)["logp"]
+    assert np.abs(logp[:period] - want).max() < 16 * U * (1 + np.abs(want).max())
+    assert np.array_equal(logp, np.tile(logp[:period], times)[:n])
+
+
+def test_the_longest_row(ctx):
+    """2^31 - 1 equal classes: every one has the same log probability, the first ones are the best."""
+    a = (1 << 31) - 1
+    s = ctx.zeros((1, a), _hip.bfloat16)
+    out = apply.log_probabilities(ctx, s, [a - 1], k=3).host()
+    want = -math.log(a)
+    assert np.array_equal(out["top_index"], [[0, 1, 2]])
+    for got in (out["logp"], out["top_logp"], -out["entropy"]):
+        assert np.abs(got - want).max() <= 8 * U * abs(want)
+
+
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n, a, kind", [(1, 1, "normal"), (4, 5, "normal"), (6, 1000, "cosine"), (5, 2500, "peaked"), (2, 9000, "normal")])
 def test_gradient_against_the_formula(ctx, n, a, kind, dt):
@@ -749,6 +774,40 @@ def test_results_do_not_change_from_call_to_call(ctx):
         got += [a.tobytes() for a in apply.log_probabilities(ctx, s, [1, 2, 3], k=9).host().values()]
         first = first or got
         assert got == first
+
+
+def test_two_threads_with_a_context_each():
+    """Each thread's forward and backward give what they give alone (contexts share no scratch)."""
+    import threading
+
+    def work(own, seed, rounds):
+        rng = np.random.default_rng(seed)
+        x, w = (own.to_device(rounded(rng.normal(size=sh), "bf16")[0]) for sh in ((400, 2001), (150, 2001)))
+        labels, ones = own.to_device(rng.integers(0, 150, 400).astype(np.int32)), own.to_device(np.ones(400, np.float32))
+        got = []
+        for _ in range(rounds):
+            y, pre = engine.linear(own, x, w, activation="silu", preact=True)
+            fwd = apply.log_probabilities(own, y, labels, k=4)
+            ds = apply.log_probabilities_backward(own, y, labels, fwd, d_logp=ones)
+            dx, dw, db = engine.linear_backward(own, ds, x, w, activation="silu", preact=pre)
+            got.append([v.download().tobytes() for v in (y, fwd.logp, fwd.top_index, dx, dw, db)])
+        return got
+
+    contexts = [_hip.Context(0) for _ in range(2)]
+    alone = [work(c, i, 1)[0] for i, c in enumerate(contexts)]
+    results = [None, None]
+
+    def thread(i):
+        results[i] = work(contexts[i], i, 25)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(60)
+    for i in range(2):
+        assert results[i] is not None and all(r == alone[i] for r in results[i])
+        contexts[i].close()
 
 
 # ---------------------------------------------------------------------------- as they are used together
