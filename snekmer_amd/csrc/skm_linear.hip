@@ -143,40 +143,66 @@ __device__ __forceinline__ void ln_read(const typename ln_type<DT>::T *from, boo
             v[u] = u < left ? from[u] : (typename ln_type<DT>::T)0.0f;
     }
 }
+// v in the type, as it is stored.  (Words that the compiler cannot look into: it would move the arithmetic behind the
+// branches of every store, each waiting for its own results.)
 template <int DT, int VE>
-__device__ __forceinline__ void ln_write(typename ln_type<DT>::T *to, bool whole, int64_t left, const float (&v)[VE])
+__device__ __forceinline__ ln_u128 ln_pack(const float (&v)[VE])
 {
     typename ln_type<DT>::T o[VE];
 #pragma unroll
     for (int u = 0; u < VE; ++u)
         o[u] = (typename ln_type<DT>::T)v[u];
-    if (whole) {
-        ln_u128 raw;
-        __builtin_memcpy(&raw, o, 16);
-        *reinterpret_cast<ln_u128 *>(to) = raw;
-    } else {
-#pragma unroll
-        for (int u = 0; u < VE; ++u)
-            if (u < left)
-                to[u] = o[u];
-    }
+    ln_u128 raw;
+    __builtin_memcpy(&raw, o, 16);
+    asm volatile("" : "+v"(raw.w[0]), "+v"(raw.w[1]), "+v"(raw.w[2]), "+v"(raw.w[3]));
+    return raw;
 }
 
-// bias, activation and residual of VE consecutive cells (i, j ..) and the stores; `left` = columns from j on
+// VE consecutive cells from (i, j) on: bias, activation and residual; the pre-activation and the output as stored
 template <int DT, int VE>
-__device__ __forceinline__ void ln_cells(const ln_gemm &g, int act, int64_t i, int64_t j, bool whole, int64_t left, const float (&bias)[VE],
-                                         const typename ln_type<DT>::T (&res)[VE], float (&v)[VE])
+struct ln_done {
+    ln_u128 z, y;
+};
+template <int DT, int VE>
+__device__ __forceinline__ ln_done<DT, VE> ln_cells(const ln_gemm &g, int act, const float (&bias)[VE], const typename ln_type<DT>::T (&res)[VE], float (&v)[VE])
 {
-    using T = typename ln_type<DT>::T;
+    ln_done<DT, VE> d;
 #pragma unroll
     for (int u = 0; u < VE; ++u)
         v[u] += bias[u];
     if (g.preact)
-        ln_write<DT, VE>((T *)g.preact + i * g.ldp + j, whole, left, v);
+        d.z = ln_pack<DT, VE>(v);
 #pragma unroll
     for (int u = 0; u < VE; ++u)
         v[u] = ln_act(act, v[u]) + (float)res[u];
-    ln_write<DT, VE>((T *)g.out + i * g.ldo + j, whole, left, v);
+    d.y = ln_pack<DT, VE>(v);
+    return d;
+}
+// `left` of them are cells of the matrix
+template <int DT, int VE>
+__device__ __forceinline__ void ln_put(const ln_gemm &g, int64_t i, int64_t j, int64_t left, const ln_done<DT, VE> &d)
+{
+    using T = typename ln_type<DT>::T;
+    T *z = (T *)g.preact + i * g.ldp + j, *y = (T *)g.out + i * g.ldo + j;
+    if (left >= VE) {
+        if (g.preact)
+            *reinterpret_cast<ln_u128 *>(z) = d.z;
+        *reinterpret_cast<ln_u128 *>(y) = d.y;
+    } else if (left > 0) {
+        T o[VE];
+        if (g.preact) {
+            __builtin_memcpy(o, &d.z, 16);
+#pragma unroll
+            for (int u = 0; u < VE; ++u)
+                if (u < left)
+                    z[u] = o[u];
+        }
+        __builtin_memcpy(o, &d.y, 16);
+#pragma unroll
+        for (int u = 0; u < VE; ++u)
+            if (u < left)
+                y[u] = o[u];
+    }
 }
 
 // calls f with the activation as a compile-time constant
@@ -289,9 +315,8 @@ __device__ __forceinline__ void ln_store_tile(const ln_gemm &g, const ln_place &
             v[u + 3] = f.w;
         }
     };
-    constexpr int UNROLL = FM > 2 ? 1 : 64;
     if constexpr (SPLIT) {
-#pragma unroll UNROLL
+#pragma unroll 1
         for (int a = 0; a < FM; ++a) {
             to_lds(a);
 #pragma unroll
@@ -333,7 +358,7 @@ __device__ __forceinline__ void ln_store_tile(const ln_gemm &g, const ln_place &
             }
         };
         fetch(0, res);
-#pragma unroll UNROLL  // (the activations' code once per 32 rows of a large tile)
+#pragma unroll 1  // (the activations' code once)
         for (int it = 0; it < FM * CHUNKS; ++it) {
             const int c = it % CHUNKS;
             if (c == 0)
@@ -341,13 +366,22 @@ __device__ __forceinline__ void ln_store_tile(const ln_gemm &g, const ln_place &
             if (g.residual && it + 1 < FM * CHUNKS)
                 fetch(it + 1, next);
             ln_with_act(g.act, [&](auto ACT) {
+                constexpr int BATCH = CHUNK < 4 ? CHUNK : 4;  // pieces worked on side by side
 #pragma unroll
-                for (int p = 0; p < CHUNK; ++p) {
-                    const int64_t i = at.row0 + wrow + (it * CHUNK + p) * ROWS + pr;
-                    float v[VE];
-                    from_lds(c * CHUNK + p, v);
-                    if (i < g.m && left > 0)
-                        ln_cells<DT, VE>(g, decltype(ACT)::value, i, j, whole, left, bias, res[p], v);
+                for (int p0 = 0; p0 < CHUNK; p0 += BATCH) {
+                    float v[BATCH][VE];
+                    ln_done<DT, VE> d[BATCH];
+#pragma unroll
+                    for (int p = 0; p < BATCH; ++p)
+                        from_lds(c * CHUNK + p0 + p, v[p]);
+#pragma unroll
+                    for (int p = 0; p < BATCH; ++p)
+                        d[p] = ln_cells<DT, VE>(g, decltype(ACT)::value, bias, res[p0 + p], v[p]);
+#pragma unroll
+                    for (int p = 0; p < BATCH; ++p) {
+                        const int64_t i = at.row0 + wrow + (it * CHUNK + p0 + p) * ROWS + pr;
+                        ln_put<DT, VE>(g, i, j, i < g.m ? left : 0, d[p]);
+                    }
                 }
             });
             if (g.residual)
@@ -765,7 +799,7 @@ __global__ __launch_bounds__(256) void k_linear_join(ln_gemm g)
 #pragma unroll
         for (int u = 0; u < VE; ++u)
             bias[u] = (float)b[u];
-        ln_with_act(g.act, [&](auto ACT) { ln_cells<DT, VE>(g, decltype(ACT)::value, i, j, whole, left, bias, res, v); });
+        ln_with_act(g.act, [&](auto ACT) { ln_put<DT, VE>(g, i, j, left, ln_cells<DT, VE>(g, decltype(ACT)::value, bias, res, v)); });
     }
 }
 
