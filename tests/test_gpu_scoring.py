@@ -652,6 +652,17 @@ def test_slopes_far_from_zero(ctx, name, dt):
     assert np.array_equal(values(y, dt)[:, 0], want)
 
 
+def test_gelu_keeps_its_precision_in_the_tail(ctx):
+    """z Phi(z) for z down to -12, relative to itself: the exponential's argument z z / 2 <= 72 has two roundings, 72 * 2^-23 in all; a
+    dozen more of float32 around it: below 2^-16."""
+    z = -np.linspace(0.5, 12.0, 301).astype(np.float32)
+    one = ctx.to_device(np.ones((1, 1), np.float32))
+    y = engine.linear(ctx, ctx.to_device(z[:, None]), one, activation="gelu").download()[:, 0].astype(np.float64)
+    z = z.astype(np.float64)
+    want = z * 0.5 * np.vectorize(math.erfc)(-z / math.sqrt(2.0))
+    assert np.abs(y / want - 1).max() < 2.0 ** -16
+
+
 def test_infinities_and_nan_stay_in_their_rows(ctx):
     x, w = whole_numbers((40, 90), 1), whole_numbers((50, 90), 2)
     w[w == 0] = 1
