@@ -927,22 +927,38 @@ __global__ __launch_bounds__(256) void k_linear_dz(int64_t rows, int64_t cols, c
     }
 }
 
-// dbias[c] = the tiles' column sums added up: a wave per 64 columns and quarter of the tiles
+// dbias[c] = the tiles' column sums added up, in one order: a wave per 64 columns and sixteenth of the tiles, eight loads under way
+// (4096 columns, 128 tiles: 11 us by four waves and a load at a time, 5 so)
 template <int DT>
-__global__ __launch_bounds__(256) void k_linear_bias_grad(int64_t parts, int64_t cols, const float *sums, void *out_)
+__global__ __launch_bounds__(1024) void k_linear_bias_grad(int64_t parts, int64_t cols, const float *sums, void *out_)
 {
     using T = typename ln_type<DT>::T;
-    __shared__ float s_sum[4][64];
+    constexpr int W = 16, AHEAD = 8;
+    __shared__ float s_sum[W][64];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
     for (int64_t c0 = (int64_t)blockIdx.x * 64; c0 < cols; c0 += (int64_t)gridDim.x * 64) {
         float v = 0.0f;
-        if (c0 + lane < cols)
-            for (int64_t p = wid; p < parts; p += 4)
-                v += sums[p * cols + c0 + lane];
+        if (c0 + lane < cols) {
+            const float *from = sums + c0 + lane;
+            for (int64_t p = wid; p < parts; p += W * AHEAD) {
+                float part[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i)
+                    part[i] = p + i * W < parts ? from[(p + i * W) * cols] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i)
+                    v += part[i];
+            }
+        }
         s_sum[wid][lane] = v;
         __syncthreads();
-        if (wid == 0 && c0 + lane < cols)
-            ((T *)out_)[c0 + lane] = (T)(s_sum[0][lane] + s_sum[1][lane] + s_sum[2][lane] + s_sum[3][lane]);
+        if (wid == 0 && c0 + lane < cols) {
+            v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                v += s_sum[i][lane];
+            ((T *)out_)[c0 + lane] = (T)v;
+        }
         __syncthreads();
     }
 }
@@ -1162,7 +1178,7 @@ int backward(skm_ctx *ctx, int act, int64_t m, int64_t n, int64_t k, const void 
             SKM_TRY(skm_check_launch("k_linear_dz"));
         }
         if (dbias) {
-            k_linear_bias_grad<DT><<<skm_grid_cap(ctx, skm_ceil_div(n, 64), 16), 256, 0, ctx->stream>>>(parts, n, (const float *)sums, dbias);
+            k_linear_bias_grad<DT><<<skm_grid_cap(ctx, skm_ceil_div(n, 64), 16), 1024, 0, ctx->stream>>>(parts, n, (const float *)sums, dbias);
             SKM_TRY(skm_check_launch("k_linear_bias_grad"));
         }
     }
