@@ -456,7 +456,8 @@ class Context:
         (skm_create_confined): a side context for work that should run beside another context's kernels.
         `stream`: the handle of a stream of the caller's (0: the null stream) that the context works on instead of one of
         its own (skm_create_on_stream), e.g. ``torch.cuda.current_stream().cuda_stream``: calls are ordered with whatever
-        its owner queues there.  The stream has to outlive the context."""
+        its owner queues there.  The stream has to outlive the context.  (Import torch before this library is first used:
+        loaded second, it brings a HIP runtime of its own that finds no device.)"""
         if stream is not None and cu_groups is not None:
             raise ValueError("a context over the caller's stream cannot be confined to compute-unit groups")
         self.lib = load_library()
