@@ -399,7 +399,8 @@ int skm_row_top2(skm_ctx *ctx, int64_t n, int64_t m, const float *d_scores, int6
  * A row without an allowed class: stats -infinity, logp -infinity, entropy 0.  A row that allows a NaN or +infinity has
  * no distribution: NaN everywhere, indices -1.  A label outside [-1, cols) gives NaN, and the next skm_sync reports it.
  * Differences of scores are taken before the temperature divides, the sums are float32, and S + 1 is never formed where
- * one class holds nearly all of the mass (log1p).  Few long rows take scratch memory. */
+ * one class holds nearly all of the mass (log1p).  Few long rows take scratch memory.  Outputs that share memory with an input or
+ * with each other are refused. */
 int skm_log_probabilities(skm_ctx *ctx, int dtype, int64_t rows, int64_t cols, const void *d_scores, int64_t ld,
                           const uint8_t *d_mask, int64_t ldmask, const void *d_labels, int label_bits, int k,
                           double temperature, float *d_logp, float *d_entropy, float *d_stats, int32_t *d_top_index,
@@ -409,7 +410,7 @@ int skm_log_probabilities(skm_ctx *ctx, int dtype, int64_t rows, int64_t cols, c
  * is not allowed.  d_grad_logp or d_grad_entropy may be NULL (0); a row with label -1 takes nothing from grad_logp, and one
  * whose label is not allowed what (j == label) - p leaves at the others: -p.  d_stats
  * (and d_entropy, with d_grad_entropy) are the forward pass's.  d_grad_scores, row stride ldg, may be d_scores itself
- * (with ldg == ld); any other overlap is refused. */
+ * (with ldg == ld); any other overlap with an input is refused. */
 int skm_log_probabilities_backward(skm_ctx *ctx, int dtype, int64_t rows, int64_t cols, const void *d_scores, int64_t ld,
                                    const uint8_t *d_mask, int64_t ldmask, const void *d_labels, int label_bits,
                                    double temperature, const float *d_stats, const float *d_entropy,
@@ -419,8 +420,8 @@ int skm_log_probabilities_backward(skm_ctx *ctx, int dtype, int64_t rows, int64_
  * all of one type (dtype 0 float32, 1 float16, 2 bfloat16), row strides in elements, any alignment; float32 sums, each output
  * rounded once.  activation 0 none, 1 relu, 2 gelu (erf), 3 gelu (tanh), 4 silu, 5 sigmoid.  d_preact [m x n] or NULL
  * receives z = x w^T + bias for the backward pass.  y may be the residual itself; any other overlap of an output with an
- * input is refused.  k = 0 is an empty sum.  Rows that do not start on 16-byte boundaries are copied to scratch first, and
- * small outputs with a long contraction are summed in parts held in scratch.  No reference counterpart in this form: the
+ * input is refused.  k = 0 is an empty sum.  16-bit rows that do not start on 4-byte boundaries (or hold an odd number) are copied
+ * to scratch first, and small outputs with a long contraction are summed in parts held in scratch.  No reference counterpart in this form: the
  * reference hands its feature matrices to scikit-learn's estimators (snekmer/model.py). */
 int skm_linear(skm_ctx *ctx, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void *d_x, int64_t ldx,
                const void *d_w, int64_t ldw, const void *d_bias, const void *d_residual, int64_t ldr, void *d_preact,

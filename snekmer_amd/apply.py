@@ -171,7 +171,7 @@ def _score_arguments(ctx, scores, labels, mask, ncols, temperature):
         raise ValueError(f"temperature: {temperature} (want a positive number)")
     mp, ldmask = None, 0
     if mask is not None:
-        two = len(mask.shape) == 2
+        two = len(getattr(mask, "shape", ())) == 2
         mp, ms, ldmask, _ = _hip.array_view(ctx, mask, "mask", 2 if two else 1, ("|u1", "|b1"))
         engine._expect("mask", ms, (rows, cols) if two else (cols,))
         ldmask = ldmask if two else 0

@@ -905,6 +905,13 @@ int lp_launch(skm_ctx *ctx, const lp_args &whole, const lp_cut &cut)
     return SKM_OK;
 }
 
+// rows of bytes
+struct lp_span {
+    const void *p;
+    int64_t rows, bytes, stride;
+};
+bool lp_share(const lp_span &a, const lp_span &b) { return skm_overlap(a.p, a.rows, a.bytes, a.stride, b.p, b.rows, b.bytes, b.stride, 1); }
+
 // what both entry points check
 int lp_check(const char *who, skm_ctx *ctx, int dtype, int64_t rows, int64_t cols, const void *d_scores, int64_t ld, const uint8_t *d_mask, int64_t ldmask,
              int label_bits, double temperature)
@@ -937,6 +944,15 @@ extern "C" int skm_log_probabilities(skm_ctx *ctx, int dtype, int64_t rows, int6
     SKM_REQUIRE(!d_logp || d_labels || rows == 0, SKM_E_BADARG, "%s: log probabilities need labels", who);
     if (rows == 0)
         return SKM_OK;
+    const int64_t es = dtype == 0 ? 4 : 2;
+    const lp_span in[3] = {{d_scores, rows, cols * es, ld * es}, {d_mask, ldmask ? rows : 1, cols, ldmask ? ldmask : cols}, {d_logp ? d_labels : nullptr, 1, rows * (label_bits / 8), rows * (label_bits / 8)}};
+    const lp_span out[5] = {{d_logp, 1, rows * 4, rows * 4}, {d_entropy, 1, rows * 4, rows * 4}, {d_stats, 1, rows * 8, rows * 8}, {d_top_index, 1, rows * k * 4, rows * k * 4}, {d_top_logp, 1, rows * k * 4, rows * k * 4}};
+    for (int o = 0; o < 5; ++o) {
+        for (const lp_span &i : in)
+            SKM_REQUIRE(!lp_share(out[o], i), SKM_E_BADARG, "%s: an output shares memory with the scores, the mask or the labels", who);
+        for (int q = 0; q < o; ++q)
+            SKM_REQUIRE(!lp_share(out[o], out[q]), SKM_E_BADARG, "%s: two outputs share memory", who);
+    }
     SKM_HIP(hipSetDevice(ctx->device));
     lp_args a = {};
     a.rows = rows;
@@ -999,6 +1015,11 @@ extern "C" int skm_log_probabilities_backward(skm_ctx *ctx, int dtype, int64_t r
     const int64_t es = dtype == 0 ? 4 : 2;
     SKM_REQUIRE((d_grad_scores == d_scores && ldg == ld) || !skm_overlap(d_grad_scores, rows, cols, ldg, d_scores, rows, cols, ld, es), SKM_E_BADARG,
                 "%s: the output shares memory with the scores without being them", who);
+    const lp_span out = {d_grad_scores, rows, cols * es, ldg * es};
+    const lp_span in[6] = {{d_mask, ldmask ? rows : 1, cols, ldmask ? ldmask : cols}, {d_grad_logp ? d_labels : nullptr, 1, rows * (label_bits / 8), rows * (label_bits / 8)}, {d_stats, 1, rows * 8, rows * 8},
+                           {d_grad_entropy ? d_entropy : nullptr, 1, rows * 4, rows * 4}, {d_grad_logp, 1, rows * 4, rows * 4}, {d_grad_entropy, 1, rows * 4, rows * 4}};
+    for (const lp_span &i : in)
+        SKM_REQUIRE(!lp_share(out, i), SKM_E_BADARG, "%s: the output shares memory with another input than the scores", who);
     SKM_HIP(hipSetDevice(ctx->device));
     lp_grad_args a = {};
     a.rows = rows;

@@ -713,6 +713,34 @@ def test_memory_shared_between_arguments(ctx):
                                          d_logp=ctx.to_device(np.ones(3, np.float32)), out=Strided(s, (3, 100), 100, 100))
 
 
+def test_log_probabilities_that_share_memory(ctx):
+    s = ctx.to_device(whole_numbers((8, 100), 1))
+    labels = ctx.to_device(np.arange(8, dtype=np.int32))
+    row = ctx.empty(8, np.float32)
+    for out in (dict(logp=row, entropy=row), dict(logp=Flat(s, 8, s.ptr + 160)), dict(logp=row, entropy=Flat(labels, 8, labels.ptr)), dict(stats=Strided(s, (8, 2), 2, 784), logp=row)):
+        with pytest.raises(_hip.HipError, match="share"):
+            apply.log_probabilities(ctx, s, labels, out=apply.LogProbabilities(**out))
+    wider = ctx.to_device(np.zeros((8, 104), np.float32))  # the columns behind the scores are free to use
+    out = Strided(wider, (8, 100), 104)
+    fwd = apply.log_probabilities(ctx, s, labels)
+    with pytest.raises(_hip.HipError, match="another input"):
+        apply.log_probabilities_backward(ctx, s, labels, fwd, d_logp=Flat(wider, 8, wider.ptr), out=out)
+    with pytest.raises(TypeError):
+        apply.log_probabilities(ctx, s, labels, mask=[1] * 100)
+
+
+class Flat:
+    """n float32 values at an address inside a DeviceArray's memory."""
+
+    def __init__(self, base, n, ptr):
+        self.base, self.shape = base, (n,)
+        self.interface = {"shape": (n,), "typestr": "<f4", "data": (ptr, False), "strides": None, "version": 2}
+
+    @property
+    def __cuda_array_interface__(self):
+        return self.interface
+
+
 # ---------------------------------------------------------------------------- streams, captures, other libraries' arrays
 def test_beside_torch():
     """Contexts over torch's streams, torch's arrays, its captures: tests/torch_interop.py, in a process that loads torch first
