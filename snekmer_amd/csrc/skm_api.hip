@@ -147,7 +147,8 @@ int create_ctx(int device_id, int first_group, int last_group, skm_ctx **out_ctx
     int n = 0;
     SKM_HIP(hipGetDeviceCount(&n));
     SKM_REQUIRE(device_id >= 0 && device_id < n, SKM_E_BADARG, "%s: device %d out of range (%d visible)", who, device_id, n);
-    SKM_HIP(hipSetDevice(device_id));
+    const skm_device_scope scope(device_id, foreign);
+    SKM_HIP(scope.err);
     hipDeviceProp_t prop;
     SKM_HIP(hipGetDeviceProperties(&prop, device_id));
     hipStream_t stream = nullptr;
@@ -245,7 +246,7 @@ extern "C" int skm_destroy(skm_ctx *ctx)
 {
     if (!ctx)
         return SKM_OK;
-    hipSetDevice(ctx->device);
+    const skm_device_scope scope(ctx->device, ctx->foreign);
     if (ctx->capturing) {  // an abandoned capture: end it so that the stream can be waited for and reused
         hipGraph_t g = nullptr;
         if (hipStreamEndCapture(ctx->stream, &g) == hipSuccess && g)
@@ -291,7 +292,7 @@ extern "C" int skm_destroy(skm_ctx *ctx)
 extern "C" int skm_event_record(skm_ctx *ctx, int slot)
 {
     SKM_REQUIRE(ctx && slot >= 0 && slot < SKM_EVENT_SLOTS, SKM_E_BADARG, "skm_event_record: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     if (ctx->user_events.empty())
         ctx->user_events.assign(SKM_EVENT_SLOTS, nullptr);
     if (!ctx->user_events[slot]) {
@@ -324,7 +325,7 @@ extern "C" int skm_stream_wait(skm_ctx *ctx, skm_ctx *src, int slot)
     SKM_REQUIRE(ctx->device == src->device, SKM_E_BADARG, "skm_stream_wait: contexts on different devices");
     if (src->user_events.empty() || !src->user_events[slot])
         return SKM_OK;  // nothing was ever recorded there: nothing to wait for
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_HIP(hipStreamWaitEvent(ctx->stream, src->user_events[slot], 0));
     return SKM_OK;
 }
@@ -377,7 +378,7 @@ extern "C" int skm_malloc(skm_ctx *ctx, size_t bytes, void **out_dptr)
 {
     SKM_REQUIRE(ctx && out_dptr, SKM_E_BADARG, "skm_malloc: null argument");
     *out_dptr = nullptr;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     return skm_pool_alloc(ctx, bytes, out_dptr);  // (skm_mem.hip: size classes, reuse behind completed events only)
 }
 
@@ -389,7 +390,7 @@ extern "C" int skm_free(skm_ctx *ctx, void *dptr)
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     if (!dptr)
         return SKM_OK;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     return skm_pool_free(ctx, dptr);
 }
 
@@ -397,7 +398,7 @@ extern "C" int skm_host_alloc(skm_ctx *ctx, size_t bytes, void **out_hptr)
 {
     SKM_REQUIRE(ctx && out_hptr, SKM_E_BADARG, "skm_host_alloc: null argument");
     *out_hptr = nullptr;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     hipError_t e = hipHostMalloc(out_hptr, bytes ? bytes : 1, hipHostMallocMapped | hipHostMallocCoherent);
     if (e != hipSuccess) {
         (void)hipGetLastError();
@@ -420,7 +421,7 @@ extern "C" int skm_host_free(skm_ctx *ctx, void *hptr)
 {
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     if (hptr) {
-        SKM_HIP(hipSetDevice(ctx->device));
+        SKM_ON_DEVICE(ctx);
         SKM_TRY(skm_quiesce_device(ctx->device));  // kernels read and write this memory in place; the wait is explicit
         SKM_HIP(hipHostFree(hptr));
     }
@@ -537,7 +538,7 @@ extern "C" int skm_graph_begin(skm_ctx *ctx)
     SKM_REQUIRE(!ctx->capturing, SKM_E_BADARG, "skm_graph_begin: a capture is already open on this context");
     SKM_REQUIRE(!ctx->foreign || ctx->stream, SKM_E_UNSUPPORTED, "skm_graph_begin: the null stream cannot be captured; use a context on another stream");
     SKM_REQUIRE(!skm_foreign_capture(ctx), SKM_E_BADARG, "skm_graph_begin: the owner of the context's stream is capturing it");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     // relaxed mode: other threads (and this one) may allocate and free while the capture is open; what is captured is
     // exactly what the library queues on this context's stream
     SKM_HIP(hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeRelaxed));
@@ -593,7 +594,7 @@ extern "C" int skm_graph_launch(skm_ctx *ctx, skm_graph *graph)
         skm_set_error("skm_graph_launch: a scratch buffer of the context was reallocated since the capture; capture again");
         return SKM_E_STALE;
     }
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_HIP(hipGraphLaunch(graph->exec, ctx->stream));
     return SKM_OK;
 }
@@ -605,7 +606,7 @@ extern "C" int skm_graph_destroy(skm_ctx *ctx, skm_graph *graph)
         return SKM_OK;
     auto it = std::find(ctx->graphs.begin(), ctx->graphs.end(), graph);
     SKM_REQUIRE(it != ctx->graphs.end(), SKM_E_BADARG, "skm_graph_destroy: not a live graph of this context");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     (void)hipStreamSynchronize(ctx->stream);  // a replay may still be running
     ctx->graphs.erase(it);
     skm_graph_release(graph);
@@ -733,7 +734,7 @@ extern "C" int skm_vectorize_csr(skm_ctx *ctx, const uint8_t *h_rank, int nsym, 
                 (long long)total_residues);
     SKM_REQUIRE(total_residues < ((int64_t)1 << 32) - 1 && n < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW,
                 "skm_vectorize_csr: more than 2^32 residues or sequences in one batch; split the batch");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     if (counts_only)
         return skm_count_stage_async(ctx, h_rank, nsym, k, code_bits, d_seq, d_off, n, total_residues, max_seq_len, d_rowptr, d_codes, d_counts,
                                      nullptr, d_rnorm, d_normsq);

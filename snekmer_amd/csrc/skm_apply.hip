@@ -491,7 +491,7 @@ extern "C" int skm_matrix_row_stats(skm_ctx *ctx, int64_t n, int64_t m, const fl
     if (n == 0)
         return SKM_OK;
     SKM_REQUIRE(d_sum && d_nnz && (m == 0 || d_in), SKM_E_BADARG, "skm_matrix_row_stats: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     const int vec_ok = (((uintptr_t)d_in & 15) == 0 && ld % 4 == 0) ? 1 : 0;
     SKM_PROF(ctx, "k_matrix_row_stats");
     k_matrix_row_stats<<<skm_grid_cap(ctx, n, 16), 256, 0, ctx->stream>>>(n, m, d_in, ld, vec_ok, d_sum, d_nnz);
@@ -511,7 +511,7 @@ extern "C" int skm_apply_top2(skm_ctx *ctx, int64_t n, const int64_t *d_xrowptr,
         return SKM_OK;
     SKM_REQUIRE(d_xrowptr && d_xnormsq && d_idx && d_score && d_dot, SKM_E_BADARG, "skm_apply_top2: null array");
     SKM_REQUIRE(m == 0 || (d_ycolptr && d_ynormsq), SKM_E_BADARG, "skm_apply_top2: null Y array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     void *p;
     SKM_TRY(skm_ws(ctx, WS_J, sizeof(double) * (size_t)(m + 1), &p));
     double *ynorm = (double *)p;
@@ -560,7 +560,7 @@ extern "C" int skm_cosine_dense_f64(skm_ctx *ctx, int64_t n, int64_t m, int64_t 
     if (n == 0 || m == 0)
         return SKM_OK;
     SKM_REQUIRE(d_x && d_y && d_out, SKM_E_BADARG, "skm_cosine_dense_f64: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     const int64_t kp = skm_ceil_div(k > 0 ? k : 1, FK) * FK;
     const bool same = d_x == d_y && ldx == ldy && n == m;
     void *p;

@@ -704,7 +704,7 @@ extern "C" int skm_basis_build(skm_ctx *ctx, int code_bits, int key_bits, int fl
     SKM_REQUIRE(d_rowptr && d_codes && d_counts && d_colidx, SKM_E_BADARG, "skm_basis_build: null CSR array");
     if (key_bits <= 0 || key_bits > code_bits)
         key_bits = code_bits;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
 #define SKM_BASIS(K, PW)                                                                                                   \
     return basis_impl<K, PW>(ctx, key_bits, flags, n, nnz, d_rowptr, (const K *)d_codes, d_counts, d_firstpos, h_ncols,  \
                              (K *)d_basis, d_colidx, d_df, d_total, d_firstkey, d_fs_order, d_colptr, (PW *)d_post, d_postcnt)
@@ -726,7 +726,7 @@ extern "C" int skm_csr_transpose(skm_ctx *ctx, int64_t n, int64_t nnz, int64_t n
     SKM_REQUIRE(ctx && d_colptr && n >= 0 && nnz >= 0 && ncols >= 0, SKM_E_BADARG, "skm_csr_transpose: bad argument");
     SKM_REQUIRE(nnz < ((int64_t)1 << 32) - 1 && ncols < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW,
                 "skm_csr_transpose: nnz or ncols >= 2^32");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     hipStream_t st = ctx->stream;
     if (nnz == 0) {
         SKM_HIP(hipMemsetAsync(d_colptr, 0, sizeof(uint32_t) * (size_t)(ncols + 1), st));
@@ -762,7 +762,7 @@ extern "C" int skm_csr_concat_rowptr(skm_ctx *ctx, int nparts, const int64_t *h_
 {
     SKM_REQUIRE(ctx && nparts >= 1 && h_nrows && h_nnz && d_local && d_rowptr, SKM_E_BADARG,
                 "skm_csr_concat_rowptr: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     int64_t src = 0, dst = 0, base = 0;
     SKM_PROF(ctx, "k_rebase_rowptr");
     for (int p = 0; p < nparts; ++p) {
@@ -787,7 +787,7 @@ extern "C" int skm_csr_to_dense(skm_ctx *ctx, int64_t n, const int64_t *d_rowptr
     if (n == 0 || ld == 0)
         return SKM_OK;
     SKM_REQUIRE(d_rowptr && d_out, SKM_E_BADARG, "skm_csr_to_dense: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     const size_t esz = dtype == 0 ? 8 : (dtype == 1 ? 4 : 1);
     SKM_HIP(hipMemsetAsync(d_out, 0, esz * (size_t)n * (size_t)ld, ctx->stream));
     const int grid = skm_grid_cap(ctx, skm_ceil_div(n, BLK / 64), 16);
@@ -811,7 +811,7 @@ extern "C" int skm_row_norms_csr(skm_ctx *ctx, int64_t n, const int64_t *d_rowpt
     if (n == 0)
         return SKM_OK;
     SKM_REQUIRE(d_rowptr, SKM_E_BADARG, "skm_row_norms_csr: null rowptr");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_PROF(ctx, "k_row_norms");
     k_row_norms<<<skm_grid_cap(ctx, skm_ceil_div(n, BLK / 64), 16), BLK, 0, ctx->stream>>>(n, d_rowptr, d_counts, d_rnorm,
                                                                                           d_normsq);
@@ -825,7 +825,7 @@ extern "C" int skm_row_top2(skm_ctx *ctx, int64_t n, int64_t m, const float *d_s
     if (n == 0)
         return SKM_OK;
     SKM_REQUIRE(d_idx && d_val && (m == 0 || d_scores), SKM_E_BADARG, "skm_row_top2: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_PROF(ctx, "k_row_top2");
     k_row_top2<<<skm_grid_cap(ctx, skm_ceil_div(n, BLK / 64), 16), BLK, 0, ctx->stream>>>(n, m, d_scores, ld, d_idx, d_val);
     return skm_check_launch("k_row_top2");
@@ -840,7 +840,7 @@ extern "C" int skm_hamming_similarity_from_gram(skm_ctx *ctx, int64_t n, int64_t
     if (n == 0 || m == 0)
         return SKM_OK;
     SKM_REQUIRE(d_xcount && d_ycount && d_out, SKM_E_BADARG, "skm_hamming_similarity_from_gram: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     dim3 grid((unsigned)skm_ceil_div(m, BLK), (unsigned)(n < 1024 ? n : 1024));
     SKM_PROF(ctx, "k_setsim_from_gram");
     k_setsim_from_gram<0><<<grid, BLK, 0, ctx->stream>>>(n, m, 1.0f / (float)ncols, d_xcount, d_ycount, d_out, ld);
@@ -854,7 +854,7 @@ extern "C" int skm_jaccard_distance_from_gram(skm_ctx *ctx, int64_t n, int64_t m
     if (n == 0 || m == 0)
         return SKM_OK;
     SKM_REQUIRE(d_xcount && d_ycount && d_out, SKM_E_BADARG, "skm_jaccard_distance_from_gram: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     dim3 grid((unsigned)skm_ceil_div(m, BLK), (unsigned)(n < 1024 ? n : 1024));
     SKM_PROF(ctx, "k_setsim_from_gram");
     k_setsim_from_gram<1><<<grid, BLK, 0, ctx->stream>>>(n, m, 0.0f, d_xcount, d_ycount, d_out, ld);
@@ -871,7 +871,7 @@ extern "C" int skm_setsim_f64(skm_ctx *ctx, int kind, int64_t n, int64_t m, int6
     if (n == 0 || m == 0)
         return SKM_OK;
     SKM_REQUIRE(d_xnnz && d_ynnz && d_both && d_out, SKM_E_BADARG, "skm_setsim_f64: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     dim3 grid((unsigned)skm_ceil_div(m, BLK), (unsigned)(n < 1024 ? n : 1024));
     SKM_PROF(ctx, "k_setsim_f64");
     if (kind == 0)
@@ -892,7 +892,7 @@ extern "C" int skm_gather_columns(skm_ctx *ctx, int64_t rows, int64_t ncols_out,
     if (rows == 0 || ncols_out == 0)
         return SKM_OK;
     SKM_REQUIRE(d_src && d_out && (ld_in == 0 || d_in), SKM_E_BADARG, "skm_gather_columns: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     dim3 grid((unsigned)skm_ceil_div(ncols_out, BLK), (unsigned)(rows < 4096 ? rows : 4096));
     SKM_PROF(ctx, "k_gather_columns");
     if (elem_bytes == 8)
@@ -912,7 +912,7 @@ extern "C" int skm_widen_i8_u32(skm_ctx *ctx, int64_t count, const int8_t *d_in,
     if (count == 0)
         return SKM_OK;
     SKM_REQUIRE(d_in && d_out, SKM_E_BADARG, "skm_widen_i8_u32: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     k_widen_i8_u32<<<skm_grid_cap(ctx, skm_ceil_div(count, BLK), 16), BLK, 0, ctx->stream>>>(count, d_in, d_out);
     return skm_check_launch("k_widen_i8_u32");
 }
@@ -923,7 +923,7 @@ extern "C" int skm_narrow_u32_u8(skm_ctx *ctx, int64_t count, const uint32_t *d_
     if (count == 0)
         return SKM_OK;
     SKM_REQUIRE(d_in && d_out, SKM_E_BADARG, "skm_narrow_u32_u8: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     k_narrow_u32_u8<<<skm_grid_cap(ctx, skm_ceil_div(count, BLK), 16), BLK, 0, ctx->stream>>>(count, d_in, d_out);
     return skm_check_launch("k_narrow_u32_u8");
 }
@@ -939,7 +939,7 @@ extern "C" int skm_csr_max_count(skm_ctx *ctx, int64_t nnz, const uint32_t *d_co
     *h_max = 0;
     if (nnz == 0)
         return SKM_OK;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     void *p;
     SKM_TRY(skm_ws(ctx, WS_SMALL, 4096, &p));
     unsigned int *acc = (unsigned int *)((uint8_t *)p + 1536);
@@ -956,7 +956,7 @@ extern "C" int skm_csr_max_count_dev(skm_ctx *ctx, int64_t n, int64_t cap_entrie
                                      const uint32_t *d_counts, uint32_t *d_out_max)
 {
     SKM_REQUIRE(ctx && n >= 0 && cap_entries >= 0 && d_rowptr && d_out_max, SKM_E_BADARG, "skm_csr_max_count_dev: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_HIP(hipMemsetAsync(d_out_max, 0, 4, ctx->stream));
     if (cap_entries == 0)
         return SKM_OK;
@@ -971,7 +971,7 @@ extern "C" int skm_pair_work(skm_ctx *ctx, int64_t ncols, const uint32_t *d_colp
     *h_pairs = 0;
     if (ncols == 0)
         return SKM_OK;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     void *p;
     SKM_TRY(skm_ws(ctx, WS_SMALL, 4096, &p));
     unsigned long long *acc = (unsigned long long *)((uint8_t *)p + 1024);

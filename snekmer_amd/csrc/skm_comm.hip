@@ -134,7 +134,7 @@ extern "C" int skm_comm_init(skm_ctx *ctx, int nranks, int rank, const uint8_t *
                 "skm_comm_init: bad argument (1 <= nranks <= %d)", SKM_MAX_RANKS);
     SKM_REQUIRE(!ctx->comm, SKM_E_BADARG, "skm_comm_init: communicator already initialised");
     SKM_TRY(load_rccl());
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     nccl_uid uid;
     memcpy(&uid, h_id, sizeof(uid));
     SKM_NCCL(g_rccl.init_rank(&ctx->comm, nranks, uid, rank));
@@ -163,7 +163,7 @@ extern "C" int skm_comm_destroy(skm_ctx *ctx)
 extern "C" int skm_allgatherv(skm_ctx *ctx, const void *d_send, const int64_t *h_bytes, void *d_recv)
 {
     SKM_REQUIRE(ctx && h_bytes && d_recv, SKM_E_BADARG, "skm_allgatherv: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     if (!ctx->comm) {
         SKM_REQUIRE(ctx->nranks == 1, SKM_E_COMM, "skm_allgatherv: communicator not initialised");
         if (h_bytes[0] > 0 && d_send != d_recv)
@@ -200,7 +200,7 @@ extern "C" int skm_alltoallv(skm_ctx *ctx, const void *d_send, const int64_t *h_
                              const int64_t *h_recv_bytes)
 {
     SKM_REQUIRE(ctx && h_send_bytes && h_recv_bytes, SKM_E_BADARG, "skm_alltoallv: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     const int nr = ctx->comm ? ctx->nranks : 1, me = ctx->comm ? ctx->rank : 0;
     SKM_REQUIRE(ctx->comm || ctx->nranks == 1, SKM_E_COMM, "skm_alltoallv: communicator not initialised");
     int64_t soff = 0, roff = 0, my_soff = 0, my_roff = 0;
@@ -294,7 +294,7 @@ extern "C" int skm_alltoallv_multi(skm_ctx *ctx, int narrays, const void *const 
                                    const int64_t *h_elem_bytes, const int64_t *h_send_counts, const int64_t *h_recv_counts)
 {
     SKM_REQUIRE(ctx && d_send && d_recv, SKM_E_BADARG, "skm_alltoallv_multi: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     skm_p2p_op ops[SKM_MAX_RANKS * SKM_MAX_ARRAYS];
     SKM_TRY(skm_plan_alltoallv(ctx->comm ? ctx->nranks : 1, narrays, h_elem_bytes, h_send_counts, h_recv_counts, ops));
     SKM_PROF(ctx, "rccl_alltoallv");
@@ -305,7 +305,7 @@ extern "C" int skm_allgatherv_multi(skm_ctx *ctx, int narrays, const void *const
                                     const int64_t *h_elem_bytes, const int64_t *h_counts)
 {
     SKM_REQUIRE(ctx && d_send && d_recv, SKM_E_BADARG, "skm_allgatherv_multi: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     skm_p2p_op ops[SKM_MAX_RANKS * SKM_MAX_ARRAYS];
     SKM_TRY(skm_plan_allgatherv(ctx->comm ? ctx->nranks : 1, ctx->comm ? ctx->rank : 0, narrays, h_elem_bytes, h_counts, ops));
     SKM_PROF(ctx, "rccl_allgatherv");

@@ -134,6 +134,29 @@ struct skm_lut256 {
     uint8_t b[256];
 };
 
+// The context's device becomes the calling thread's current one.  Contexts over a caller's stream give it back when the call
+// ends: their owner (a program on several devices, another library that asks the runtime where it is) keeps its own.
+struct skm_device_scope {
+    int before = -1;
+    hipError_t err = hipSuccess;
+    skm_device_scope(int device, bool foreign)
+    {
+        if (foreign && (hipGetDevice(&before) != hipSuccess || before == device))
+            before = -1;
+        err = hipSetDevice(device);
+    }
+    ~skm_device_scope()
+    {
+        if (before >= 0)
+            (void)hipSetDevice(before);
+    }
+    skm_device_scope(const skm_device_scope &) = delete;
+    skm_device_scope &operator=(const skm_device_scope &) = delete;
+};
+#define SKM_ON_DEVICE(ctx)                                              \
+    const skm_device_scope skm_scope_((ctx)->device, (ctx)->foreign);   \
+    SKM_HIP(skm_scope_.err)
+
 static inline int64_t skm_ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Whether the cells of [ra x ca] at a (row stride lda) and [rb x cb] at b can share memory.  Column blocks of one matrix

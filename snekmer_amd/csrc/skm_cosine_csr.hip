@@ -1394,7 +1394,7 @@ int gram_neighbors_impl(skm_ctx *ctx, int64_t n, const int64_t *d_xrowptr, const
         return SKM_OK;
     SKM_REQUIRE(d_xrowptr && d_ycolptr && d_start && d_len && d_xrnorm && d_yrnorm && (cap_ent == 0 || d_ent), SKM_E_BADARG,
                 "skm_gram_neighbors: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     hipStream_t st = ctx->stream;
     void *p;
     SKM_TRY(skm_ws(ctx, WS_E, sizeof(uint32_t) * (size_t)(nrows + 8), &p));
@@ -1482,7 +1482,7 @@ extern "C" int skm_neighbors_topk(skm_ctx *ctx, int64_t nrows, int64_t row0, con
     if (nrows == 0)
         return SKM_OK;
     SKM_REQUIRE(d_start && d_len && d_xrnorm && d_yrnorm && d_idx && d_val, SKM_E_BADARG, "skm_neighbors_topk: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     if (k <= TOPK_KREG) {  // one pass per row, the lanes' best in registers
         // max_j yrnorm[j] for the bound that spares the gather of hopeless entries' norms (m <= 0: the caller did not say
         // how many norms there are: +infinity, every norm is gathered)
@@ -1729,7 +1729,7 @@ int cosine_csr_impl(skm_ctx *ctx, int64_t n, const int64_t *d_xrowptr, const uin
     if (row1 == row0 || m == 0)
         return SKM_OK;
     SKM_REQUIRE(d_xrowptr && d_xrnorm && d_ycolptr && d_yrnorm && (d_out || phase == 1), SKM_E_BADARG, "skm_cosine_csr: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     const int64_t nrows = row1 - row0;
     const int64_t strips = skm_ceil_div(nrows, R);
     SKM_REQUIRE(strips < ((int64_t)1 << 31), SKM_E_OVERFLOW, "skm_cosine_csr: too many rows in one call");
@@ -2038,7 +2038,7 @@ extern "C" int skm_cosine_csr_stats(skm_ctx *ctx, int64_t *h_out4)
     h_out4[0] = h_out4[1] = h_out4[2] = h_out4[3] = 0;
     if (!ctx->ws[WS_COS] || ctx->ws_bytes[WS_COS] < sizeof(cos_state))
         return SKM_OK;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     cos_state host;
     SKM_HIP(hipMemcpyAsync(&host, ctx->ws[WS_COS], offsetof(cos_state, pad), hipMemcpyDeviceToHost, ctx->stream));
     SKM_HIP(hipStreamSynchronize(ctx->stream));
@@ -2060,7 +2060,7 @@ extern "C" int skm_heavy_panel_stats(skm_ctx *ctx, int64_t *h_out6)
         h_out6[q] = 0;
     if (!ctx->panel_meta || ctx->panel_nb <= 0)
         return SKM_OK;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     std::vector<uint32_t> meta(4 * (size_t)ctx->panel_nb);
     uint32_t rows = 0;

@@ -1037,7 +1037,7 @@ extern "C" int skm_count_dense(skm_ctx *ctx, const uint8_t *h_rank, int nsym, in
     if (n == 0)
         return SKM_OK;
     SKM_REQUIRE(d_out && d_seq, SKM_E_BADARG, "skm_count_dense: null buffer");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     skm_lut256 lut;
     memcpy(lut.b, h_rank, 256);
     const size_t cell = dtype == 0 ? 2 : 4;
@@ -1093,7 +1093,7 @@ static int cosine_dense_i8_impl(skm_ctx *ctx, int64_t n, int64_t m, int64_t kdim
         return SKM_OK;
     SKM_REQUIRE(d_x && d_y && d_xrnorm && d_yrnorm && d_out, SKM_E_BADARG, "skm_cosine_dense_i8: null array");
     SKM_REQUIRE((((uintptr_t)d_x | (uintptr_t)d_y) & 15) == 0, SKM_E_BADARG, "skm_cosine_dense_i8: operands must be 16-byte aligned");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     if (kdim * 127 * 127 >= ((int64_t)1 << 31)) {
         // Wider than 133 143 columns, 127^2 * kdim no longer bounds the int32 accumulators: the norms must
         // (<x, y> <= 1 / (xrnorm * yrnorm), the test of skm_cosine_csr).  Rare shape, so this one waits for the device.
@@ -1278,7 +1278,7 @@ extern "C" int skm_dense_to_csr(skm_ctx *ctx, int64_t n, int64_t ncols, int dtyp
                 "skm_dense_to_csr: bad argument");
     SKM_REQUIRE(dtype >= 0 && dtype <= 2, SKM_E_BADARG, "skm_dense_to_csr: dtype must be 0 (uint16), 1 (uint32) or 2 (int8)");
     SKM_REQUIRE(ncols < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW, "skm_dense_to_csr: ncols >= 2^32");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     hipStream_t st = ctx->stream;
     *h_nnz = 0;
     if (n == 0 || ncols == 0) {
@@ -1341,7 +1341,7 @@ extern "C" int skm_row_norms_i8(skm_ctx *ctx, int64_t n, int64_t kdim, const int
     if (n == 0)
         return SKM_OK;
     SKM_REQUIRE(d_in && ((uintptr_t)d_in & 15) == 0, SKM_E_BADARG, "skm_row_norms_i8: matrix must be 16-byte aligned");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_PROF(ctx, "k_row_norms_i8");
     k_row_norms_i8<<<skm_grid_cap(ctx, skm_ceil_div(n, 4), 16), 256, 0, ctx->stream>>>(n, kdim, d_in, d_rnorm, d_normsq);
     return skm_check_launch("k_row_norms_i8");
@@ -1465,7 +1465,7 @@ extern "C" int skm_csr_to_dense_i8(skm_ctx *ctx, int64_t n, const int64_t *d_row
 {
     SKM_REQUIRE(ctx && n >= 0 && kdim >= 0 && kdim % 64 == 0, SKM_E_BADARG, "skm_csr_to_dense_i8: bad argument (kdim must be a multiple of 64)");
     SKM_REQUIRE(d_irr_count, SKM_E_BADARG, "skm_csr_to_dense_i8: null counter");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_HIP(hipMemsetAsync(d_irr_count, 0, sizeof(uint32_t), ctx->stream));
     if (n == 0 || kdim == 0)
         return SKM_OK;
@@ -1486,7 +1486,7 @@ extern "C" int skm_cosine_fixup_rows(skm_ctx *ctx, int64_t n, const int64_t *d_r
         return SKM_OK;
     SKM_REQUIRE(d_rowptr && d_codes && d_counts && d_rnorm && d_irr_list && d_irr_count && d_out, SKM_E_BADARG,
                 "skm_cosine_fixup_rows: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_PROF(ctx, "k_cosine_fixup_rows");
     const int grid = skm_grid_cap(ctx, n, 4);  // strides over (irregular rows) x (chunks of 256 rows); empty list: exits at once
     if (mode == 0)

@@ -158,7 +158,7 @@ extern "C" int skm_rows_to_utf32(skm_ctx *ctx, const uint8_t *d_bytes, const int
     if (n == 0)
         return SKM_OK;
     SKM_REQUIRE(d_bytes && d_off && d_len && d_out, SKM_E_BADARG, "skm_rows_to_utf32: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_PROF(ctx, "k_rows_to_utf32");
     k_rows_to_utf32<<<skm_grid_cap(ctx, skm_ceil_div(n, BLK / 64), 16), BLK, 0, ctx->stream>>>(d_bytes, d_off, d_len, n, width, d_out);
     return skm_check_launch("k_rows_to_utf32");
@@ -176,7 +176,7 @@ extern "C" int skm_decode_kmers_utf32(skm_ctx *ctx, int code_bits, int nsym, int
     letters64 lt = {};
     for (int s = 0; s < nsym; ++s)
         lt.c[s] = h_letters[s];
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     const size_t lds = sizeof(uint32_t) * BLK * (size_t)k;
     const int grid = skm_grid_cap(ctx, skm_ceil_div(n, BLK), 16);
     SKM_PROF(ctx, "k_decode_kmers_utf32");
@@ -192,7 +192,7 @@ extern "C" int skm_csr_remap_columns(skm_ctx *ctx, int64_t n, const int64_t *d_r
                                      uint32_t *d_out_col, uint32_t *d_out_val, int64_t *h_out_nnz)
 {
     SKM_REQUIRE(ctx && n >= 0 && ncols >= 0 && d_out_rowptr && h_out_nnz, SKM_E_BADARG, "skm_csr_remap_columns: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     hipStream_t st = ctx->stream;
     *h_out_nnz = 0;
     if (n == 0) {
@@ -239,7 +239,7 @@ extern "C" int skm_basis_select(skm_ctx *ctx, int64_t ncols, const uint32_t *d_f
     if (ncols == 0)
         return SKM_OK;
     SKM_REQUIRE(d_fs_order && d_total && d_keep && d_colmap, SKM_E_BADARG, "skm_basis_select: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     hipStream_t st = ctx->stream;
     void *p;
     SKM_TRY(skm_ws(ctx, WS_A, sizeof(uint32_t) * (size_t)ncols, &p));

@@ -956,7 +956,7 @@ extern "C" int skm_recode(skm_ctx *ctx, const uint8_t *h_translate, const uint8_
     SKM_TRY(make_lut(h_translate, &lut));
     if (n == 0)
         return SKM_OK;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     int64_t *h_tot = (int64_t *)ctx->h_pinned;
     SKM_HIP(hipMemcpyAsync(h_tot, d_off + n, sizeof(int64_t), hipMemcpyDeviceToHost, ctx->stream));
     SKM_HIP(hipStreamSynchronize(ctx->stream));
@@ -988,7 +988,7 @@ extern "C" int skm_kmer_codes(skm_ctx *ctx, const uint8_t *h_rank, int nsym, int
     SKM_TRY(check_code_space(nsym, k, code_bits));
     if (n == 0)
         return SKM_OK;
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     void *p;
     SKM_TRY(skm_ws(ctx, WS_A, sizeof(int32_t) * (size_t)(n + 1), &p));
     int32_t *slen = (int32_t *)p;
@@ -1022,7 +1022,7 @@ extern "C" int skm_count_csr(skm_ctx *ctx, const uint8_t *h_rank, int nsym, int 
     skm_lut256 lut;
     SKM_TRY(make_lut(h_rank, &lut));
     SKM_TRY(check_code_space(nsym, k, code_bits));
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     *h_nnz = 0;
     if (n == 0) {
         SKM_HIP(hipMemsetAsync(d_rowptr, 0, sizeof(int64_t), ctx->stream));

@@ -378,7 +378,7 @@ extern "C" int skm_group_postings(skm_ctx *ctx, int64_t n, int64_t ncols, const 
                 "skm_group_postings: bad argument");
     SKM_REQUIRE(nnz < ((int64_t)1 << 32) - 1 && ncols < ((int64_t)1 << 32) - 1 && ngroups < ((int64_t)1 << 32) - 2, SKM_E_OVERFLOW,
                 "skm_group_postings: too large");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     hipStream_t st = ctx->stream;
     *h_out_nnz = 0;
     if (d_out_normsq && ngroups)
@@ -436,7 +436,7 @@ extern "C" int skm_postings_to_csr(skm_ctx *ctx, int64_t ncols, int64_t nnz, con
 {
     SKM_REQUIRE(ctx && ncols >= 0 && nnz >= 0 && nrows >= 0 && d_out_rowptr, SKM_E_BADARG, "skm_postings_to_csr: bad argument");
     SKM_REQUIRE(nnz < ((int64_t)1 << 32) - 1 && nrows < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW, "skm_postings_to_csr: too large");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     hipStream_t st = ctx->stream;
     if (nnz == 0) {
         SKM_HIP(hipMemsetAsync(d_out_rowptr, 0, sizeof(int64_t) * (size_t)(nrows + 1), st));
@@ -496,7 +496,7 @@ extern "C" int skm_csr_group_sum(skm_ctx *ctx, int64_t n, int64_t nnz, const int
     SKM_REQUIRE(ctx && n >= 0 && nnz >= 0 && ngroups >= 0 && d_out_rowptr && h_out_nnz, SKM_E_BADARG,
                 "skm_csr_group_sum: bad argument");
     SKM_REQUIRE(nnz < ((int64_t)1 << 32) - 1 && ngroups < ((int64_t)1 << 32) - 2, SKM_E_OVERFLOW, "skm_csr_group_sum: too large");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     hipStream_t st = ctx->stream;
     *h_out_nnz = 0;
     if (nnz == 0) {

@@ -43,7 +43,7 @@ extern "C" int skm_linear(skm_ctx *ctx, int dtype, int activation, int64_t m, in
                     "%s: an output shares memory with the residual without being it", who);
     }
     SKM_REQUIRE(!skm_overlap(d_y, m, n, ldy, d_preact, m, n, ldp, es), SKM_E_BADARG, "%s: y and preact share memory", who);
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     if (dtype == 0)
         return skm_linear_forward<0>(ctx, activation, m, n, k, d_x, ldx, d_w, ldw, d_bias, d_residual, ldr, d_preact, ldp, d_y, ldy);
     if (dtype == 1)
@@ -93,7 +93,7 @@ extern "C" int skm_linear_backward(skm_ctx *ctx, int dtype, int activation, int6
             SKM_REQUIRE(!skm_overlap(out[o].p, out[o].rows, out[o].cols, out[o].ld, out[q].p, out[q].rows, out[q].cols, out[q].ld, es), SKM_E_BADARG,
                         "%s: two gradients share memory", who);
     }
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     // (k = 0: dx and dw have no cells, the bias's gradient is what is left; m or n = 0: what has cells is an empty sum)
     void *dx = m && k ? d_dx : nullptr, *dw = n && k ? d_dw : nullptr, *db = n ? d_dbias : nullptr;
     if (!dx && !dw && !db)

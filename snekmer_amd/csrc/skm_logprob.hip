@@ -953,7 +953,7 @@ extern "C" int skm_log_probabilities(skm_ctx *ctx, int dtype, int64_t rows, int6
         for (int q = 0; q < o; ++q)
             SKM_REQUIRE(!lp_share(out[o], out[q]), SKM_E_BADARG, "%s: two outputs share memory", who);
     }
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     lp_args a = {};
     a.rows = rows;
     a.cols = cols;
@@ -1020,7 +1020,7 @@ extern "C" int skm_log_probabilities_backward(skm_ctx *ctx, int dtype, int64_t r
                            {d_grad_entropy ? d_entropy : nullptr, 1, rows * 4, rows * 4}, {d_grad_logp, 1, rows * 4, rows * 4}, {d_grad_entropy, 1, rows * 4, rows * 4}};
     for (const lp_span &i : in)
         SKM_REQUIRE(!lp_share(out, i), SKM_E_BADARG, "%s: the output shares memory with another input than the scores", who);
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     lp_grad_args a = {};
     a.rows = rows;
     a.cols = cols;

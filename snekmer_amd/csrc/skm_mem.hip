@@ -514,7 +514,7 @@ int skm_pool_free(skm_ctx *ctx, void *ptr)
 extern "C" int skm_mem_trim(skm_ctx *ctx, int64_t *h_released_bytes)
 {
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     device_pool *p = pool_of(ctx->device);
     SKM_REQUIRE(p, SKM_E_BADARG, "skm_mem_trim: device %d out of range", ctx->device);
     std::lock_guard<std::timed_mutex> lock(p->mu);

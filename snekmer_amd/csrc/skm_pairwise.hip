@@ -160,7 +160,7 @@ extern "C" int skm_pairwise_f64(skm_ctx *ctx, int metric, double p, int64_t n, i
     if (n == 0 || m == 0)
         return SKM_OK;
     SKM_REQUIRE(d_x && d_y && d_out, SKM_E_BADARG, "skm_pairwise_f64: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     const int square = d_x == d_y && n == m && ldx == ldy;
     dim3 grid((unsigned)skm_ceil_div(m, PT), (unsigned)skm_ceil_div(n, PT));
     SKM_PROF(ctx, "k_pairwise_f64");

@@ -353,7 +353,7 @@ extern "C" int skm_bucket_partition(skm_ctx *ctx, int code_bits, int nbuckets, i
                 SKM_MAX_RANKS);
     SKM_REQUIRE(cap_entries < ((int64_t)1 << 30) && row_base + n < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW,
                 "skm_bucket_partition: 2^30 entries or more in one shard, or a row index >= 2^32");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     if (h_counts)
         for (int b = 0; b < nbuckets; ++b)
             h_counts[b] = 0;
@@ -414,7 +414,7 @@ extern "C" int skm_bucket_postings(skm_ctx *ctx, int code_bits, int key_bits, in
     SKM_REQUIRE(nrecv < ((int64_t)1 << 31), SKM_E_OVERFLOW, "skm_bucket_postings: more than 2^31 entries for one owner");
     SKM_REQUIRE((d_tab_keys && d_tab_vals) || (!d_tab_keys && !d_tab_vals && d_ret), SKM_E_BADARG,
                 "skm_bucket_postings: give the table (keys and values), the answer array d_ret, or both");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     if (nrecv == 0) {
         k_empty_owner<<<1, 1, 0, ctx->stream>>>(d_out4, d_tab_vals);
         SKM_TRY(skm_check_launch("k_empty_owner"));
@@ -438,7 +438,7 @@ extern "C" int skm_concat_colptr(skm_ctx *ctx, int nparts, const int64_t *h_ncol
                                  const uint32_t *d_starts, uint32_t *d_colptr)
 {
     SKM_REQUIRE(ctx && nparts >= 1 && h_ncols && h_npost && d_colptr, SKM_E_BADARG, "skm_concat_colptr: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     int64_t col = 0, base = 0;
     SKM_PROF(ctx, "k_rebase_u32");
     for (int p = 0; p < nparts; ++p) {
@@ -482,7 +482,7 @@ extern "C" int skm_colidx_lookup(skm_ctx *ctx, int code_bits, int nbuckets, int6
     seg.slot[nbuckets] = (uint32_t)slot;
     seg.col[nbuckets] = (uint32_t)col;
     SKM_REQUIRE(d_codes && d_colidx && (slot == 0 || (d_tab_keys && d_tab_vals)), SKM_E_BADARG, "skm_colidx_lookup: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_PROF(ctx, "k_colidx_lookup");
     const int grid = skm_grid_cap(ctx, skm_ceil_div(nnz, BLK), 16);
     if (code_bits == 32)
@@ -515,7 +515,7 @@ extern "C" int skm_colidx_from_owners(skm_ctx *ctx, int nbuckets, int64_t nnz, c
     if (nnz == 0)
         return SKM_OK;
     SKM_REQUIRE(d_back && d_index && d_colidx, SKM_E_BADARG, "skm_colidx_from_owners: null array");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_PROF(ctx, "k_colidx_from_owners");
     k_colidx_from_owners<<<skm_grid_cap(ctx, skm_ceil_div(nnz, BLK), 16), BLK, 0, ctx->stream>>>(nnz, nbuckets, grp, d_back, d_index,
                                                                                                  d_colidx);
@@ -527,7 +527,7 @@ extern "C" int skm_embed_rowptr(skm_ctx *ctx, int64_t n_total, int64_t lo, int64
 {
     SKM_REQUIRE(ctx && n_total >= 0 && lo >= 0 && nloc >= 0 && lo + nloc <= n_total && d_local && d_rowptr, SKM_E_BADARG,
                 "skm_embed_rowptr: bad argument");
-    SKM_HIP(hipSetDevice(ctx->device));
+    SKM_ON_DEVICE(ctx);
     SKM_PROF(ctx, "k_embed_rowptr");
     k_embed_rowptr<<<(unsigned)skm_ceil_div(n_total + 1, BLK), BLK, 0, ctx->stream>>>(n_total, lo, nloc, d_local, d_rowptr);
     return skm_check_launch("k_embed_rowptr");
