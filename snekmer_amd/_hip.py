@@ -391,12 +391,12 @@ def array_view(ctx: "Context", x, name: str, ndim: int, types, writable: bool = 
         # Tensors whose dtype has come through the interface before answer its questions one by one in half a microsecond;
         # building the interface's dictionary takes them two, and a call passes up to seven arrays.
         try:
-            typestr = _TENSOR_TYPES[x.dtype]
-            fast = x.is_cuda and not x.requires_grad
+            typestr, device = _TENSOR_TYPES[x.dtype], x.get_device()
+            fast = device >= 0 and not x.requires_grad
         except (AttributeError, KeyError, TypeError):
             fast = False
         if fast:
-            ptr, shape, strides, device = x.data_ptr(), x.shape, x.stride(), x.device.index
+            ptr, shape, strides = x.data_ptr(), x.shape, x.stride()
         else:
             ptr, shape, strides, device, typestr = _from_interface(ctx, x, name, writable)
     if typestr not in types:
@@ -441,7 +441,7 @@ def _from_interface(ctx: "Context", x, name: str, writable: bool):
     if strides is not None:
         size = _ITEMSIZE.get(typestr, 1)
         strides = tuple(s // size if s % size == 0 else s / size for s in strides)
-    if typestr in _ITEMSIZE and all(hasattr(x, a) for a in ("data_ptr", "stride", "is_cuda", "requires_grad", "dtype")):
+    if typestr in _ITEMSIZE and all(hasattr(x, a) for a in ("data_ptr", "stride", "get_device", "requires_grad", "dtype")):
         _TENSOR_TYPES[x.dtype] = typestr
     return ptr, shape, strides, device, typestr
 
