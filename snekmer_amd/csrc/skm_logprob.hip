@@ -28,6 +28,7 @@
 #include <cmath>
 
 #include "skm_common.h"
+#include "skm_logprob.h"
 
 namespace {
 
@@ -807,15 +808,15 @@ __global__ __launch_bounds__(256) void k_log_probabilities_grad(lp_grad_args a)
             x[e] = x[e] == -LP_INF ? 0.0f : r;
         }
         // the label's entry again, by the lane that holds it
-        const int64_t off = y - base;
-        if (y >= 0 && off >= 0 && off < LP_TILE && (int)((off / VE) & 63) == lane) {
+        const int off = lp_entry_of(y, base, rem);
+        if (off >= 0 && ((off / VE) & 63) == lane) {
             const float s = P::one(srow[y]);
             const bool allowed = s != -LP_INF && (!MASK || a.mask[row * a.ldmask + y] != 0);
             const float z = (s - m) * a.inv_t - l;
             const float d = allowed ? -gi * expm1f(z) - __builtin_amdgcn_exp2f(z * 1.44269504088896f) * hi * (fmaxf((s - m) * a.inv_t, -1e30f) + hl) : 0.0f;
 #pragma unroll
             for (int e = 0; e < LP_E; ++e)
-                if ((int)off / VE / 64 == e / VE && (int)off - lp_start<VE>(e / VE, lane, rem) == e % VE)
+                if (off / VE / 64 == e / VE && off - lp_start<VE>(e / VE, lane, rem) == e % VE)
                     x[e] = d;
         }
 #pragma unroll

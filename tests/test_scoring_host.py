@@ -1,0 +1,59 @@
+"""Parts of the scoring operators that can be checked without a device: index arithmetic of the kernels compiled for the host, and
+what the library's sources and Python layer promise about streams, devices and arguments."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "snekmer_amd", "csrc")
+
+
+def run_on_host(tmp_path, source):
+    """Compiles a program against the kernels' headers and runs it: its output."""
+    if shutil.which("g++") is None:
+        pytest.skip("no g++ here")
+    path = tmp_path / "check.cpp"
+    path.write_text(source)
+    program = str(tmp_path / "check")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", f"-I{CSRC}", str(path), "-o", program], check=True)
+    return subprocess.run([program], capture_output=True, text=True, check=True, timeout=60).stdout
+
+
+def test_a_labels_entry_is_inside_its_row(tmp_path):
+    """Every tile of rows of 1 .. 2100 classes, labels from below 0 to a tile behind the row and far ones: a label that is a class is
+    found in exactly one tile, at its place; one that is not is found in none, so that nothing is read at it."""
+    out = run_on_host(tmp_path, r"""
+#include <algorithm>
+#include <cstdio>
+#include "skm_logprob.h"
+int main()
+{
+    const int64_t tile = 1024, far[] = {INT64_MIN, INT64_MIN + 1, -(1LL << 40), -2, 1LL << 31, 1LL << 32, (1LL << 32) + 5, 1LL << 40, INT64_MAX};
+    long looked = 0;
+    for (int64_t cols = 1; cols <= 2100; cols += cols < 40 || (cols > 990 && cols < 1060) || cols > 2030 ? 1 : 37) {
+        auto check = [&](int64_t y) {
+            int found = 0;
+            for (int64_t base = 0; base < cols; base += tile) {
+                const int off = lp_entry_of(y, base, (int)std::min(tile, cols - base));
+                if (off < 0)
+                    continue;
+                ++found;
+                if (base + off != y || y >= cols)
+                    return false;
+            }
+            ++looked;
+            return found == (y >= 0 && y < cols);
+        };
+        for (int64_t y = -3; y < cols + tile + 3; ++y)
+            if (!check(y))
+                return std::printf("label %lld of %lld\n", (long long)y, (long long)cols), 1;
+        for (int64_t y : far)
+            if (!check(y))
+                return std::printf("label %lld of %lld\n", (long long)y, (long long)cols), 1;
+    }
+    std::printf("looked at %ld\n", looked);
+}
+""")
+    assert int(out.split()[-1]) > 100000
