@@ -798,13 +798,16 @@ __global__ __launch_bounds__(256) void k_log_probabilities_grad(lp_grad_args a)
         const float gl = wrong ? __builtin_nanf("") : y >= 0 ? a.d_logp[row] : 0.0f;
         const float gh = a.d_entropy ? a.d_entropy[row] : 0.0f;
         const float m = a.stats[2 * row], l = a.stats[2 * row + 1], hl = (a.d_entropy ? a.entropy[row] : 0.0f) - l;
-        const float l2 = l * 1.44269504088896f, gi = gl * a.inv_t, hi = gh * a.inv_t;
+        const float l2 = l * 1.44269504088896f;
+        // p is 0 in float32 from d = -104 on (l is not negative), however far the scaled difference goes: cut off at -1000 it
+        // changes no product, and gh times it stays finite for every gh below 3e35 - 0 times infinity would be NaN.  1 / T comes
+        // last for the same reason: gh / T times it need not be finite.
+        auto far = [](float d) { return fmaxf(d, -1e3f); };
 #pragma unroll
         for (int e = 0; e < LP_E; ++e) {
             const float t = x[e] - m;
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(t, a.c2, -l2));
-            // (p is 0 where the scaled difference is beyond float32: the clamp keeps 0 times infinity out)
-            const float r = -p * __builtin_fmaf(hi, fmaxf(t * a.inv_t, -1e30f) + hl, gi);
+            const float r = -p * __builtin_fmaf(gh, far(t * a.inv_t) + hl, gl) * a.inv_t;
             x[e] = x[e] == -LP_INF ? 0.0f : r;
         }
         // the label's entry again, by the lane that holds it
@@ -813,7 +816,8 @@ __global__ __launch_bounds__(256) void k_log_probabilities_grad(lp_grad_args a)
             const float s = P::one(srow[y]);
             const bool allowed = s != -LP_INF && (!MASK || a.mask[row * a.ldmask + y] != 0);
             const float z = (s - m) * a.inv_t - l;
-            const float d = allowed ? -gi * expm1f(z) - __builtin_amdgcn_exp2f(z * 1.44269504088896f) * hi * (fmaxf((s - m) * a.inv_t, -1e30f) + hl) : 0.0f;
+            const float p = __builtin_amdgcn_exp2f(z * 1.44269504088896f);
+            const float d = allowed ? -(gl * expm1f(z) + p * gh * (far((s - m) * a.inv_t) + hl)) * a.inv_t : 0.0f;
 #pragma unroll
             for (int e = 0; e < LP_E; ++e)
                 if (off / VE / 64 == e / VE && off - lp_start<VE>(e / VE, lane, rem) == e % VE)

@@ -48,3 +48,74 @@ def test_gradient_of_rows_with_wrong_labels(ctx, a, masked, dt):
     bad = right != labels
     assert np.isnan(got[bad][allowed[bad]]).all() and (got[bad][~allowed[bad]] == 0).all()
     assert np.array_equal(got[~bad], want[~bad])
+
+
+# ---------------------------------------------------------------------------- gradients and scores of extreme size
+def exact_gradient(want, labels, gl, gh, T):
+    """[gl ((j == y) - p_j) - gh p_j (z_j + H)] / T in 64 bits; p z is 0 where p is."""
+    z, p, h = np.where(want["p"] > 0, want["z"], 0.0), want["p"], want["entropy"][:, None]
+    known = labels >= 0
+    g = np.where(known, gl, 0.0)
+    out = -g[:, None] * p - gh[:, None] * p * (z + h)
+    at = np.flatnonzero(known), labels[known]
+    out[at] += g[known] * (p[at] - np.expm1(want["z"][at]))
+    return out / T
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T", [0.05, 1.0])
+def test_entropy_gradient_of_large_size_beside_classes_at_the_types_lowest_value(ctx, dt, T):
+    """Classes that a mask filled with the type's lowest value have p = 0 in any precision, and no part in the gradient, however large the
+    gradient that comes in (2^25: a scaled loss; 2^80); the label may be one of them.  p is off by (4 |d| + 4 l + 8) u relative, d the scaled
+    difference below 2^8 here where p is not 0, plus what l and H are off: 2^-13 of the terms covers them.  p below 2^-126 may be 0."""
+    lowest = {"f32": np.finfo(np.float32).min, "f16": -65504.0, "bf16": -3.3895313892515355e38}[dt]
+    rng = np.random.default_rng(5)
+    n, a = 6, 1500
+    s = rng.normal(size=(n, a))
+    s[rng.random((n, a)) < 0.5] = lowest
+    s[3] = lowest
+    s[3, 700] = 1.0  # one class is left
+    s[4] = lowest    # all of them alike
+    words, s = rounded(s, dt)
+    labels = np.array([0, -1, 1499, 700, 3, 5])
+    labels[5] = np.flatnonzero(s[5] == s[5].min())[0]  # (a class that the mask filled)
+    want = plain_logp(s, labels, 0, T)
+    d = ctx.to_device(words)
+    fwd = apply.log_probabilities(ctx, d, labels, temperature=T)
+    for size in (2.0 ** 25, 2.0 ** 80) if dt != "f16" else (2.0 ** 7,):
+        gl, gh = rng.normal(size=n).astype(np.float32), (size * rng.normal(size=n)).astype(np.float32)
+        for use_l in (True, False):
+            g = gl.astype(np.float64) * use_l
+            got = values(apply.log_probabilities_backward(ctx, d, labels, fwd, d_logp=ctx.to_device(gl) if use_l else None, d_entropy=ctx.to_device(gh),
+                                                          temperature=T).download(), dt)
+            exact = exact_gradient(want, labels, g, gh.astype(np.float64), T)
+            z = np.where(want["p"] > 0, want["z"], 0.0)
+            weight = (np.abs(g)[:, None] + np.abs(gh.astype(np.float64))[:, None] * (np.abs(z) + want["entropy"][:, None] + 1.0)) / T
+            terms = want["p"] * weight + np.abs(g)[:, None] * (np.arange(a) == labels[:, None]) / T
+            assert (np.abs(got - exact) <= 2.0 ** -13 * terms + 2.0 ** -125 * weight + HALF_STEP[dt] * np.abs(exact) * 1.01 + SMALLEST[dt]).all()
+            gone = (want["p"] == 0) & (np.arange(a) != labels[:, None])
+            assert gone[:4].any() and (got[gone] == 0).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [1e-20, 1e-29])
+def test_gradients_at_temperatures_near_nothing(ctx, dt, T):
+    """Everything is on the largest score: H = 0 and p is 0 or 1, so the entropy's gradient is 0 and the label's is +-gl / T (two roundings
+    of float32: 1 / T and the product)."""
+    rng = np.random.default_rng(8)
+    words, s = rounded(np.stack([rng.permutation(700) / 64.0 - 3.0 for _ in range(5)]), dt)  # (steps of 1 / 64: distinct in float32)
+    if dt == "bf16":
+        s[:, 0], words[:, 0] = 20.0, rounded(np.full(5, 20.0), dt)[0]  # (the largest one, once)
+    labels = np.array([3, -1, 0, 699, 5])
+    labels[4] = s[4].argmax()
+    gl, gh = rng.normal(size=5).astype(np.float32), rng.normal(size=5).astype(np.float32)
+    d = ctx.to_device(words)
+    fwd = apply.log_probabilities(ctx, d, labels, temperature=T)
+    assert (fwd.entropy.download() == 0).all()
+    got = values(apply.log_probabilities_backward(ctx, d, labels, fwd, d_logp=ctx.to_device(gl), d_entropy=ctx.to_device(gh), temperature=T).download(), dt)
+    exact = np.zeros((5, 700))
+    for i, y in enumerate(labels):
+        if y >= 0:
+            exact[i, y] += gl[i] / T
+            exact[i, s[i].argmax()] -= gl[i] / T
+    assert (np.abs(got - exact) <= (4 * U + HALF_STEP[dt] * 1.01) * np.abs(exact)).all()
