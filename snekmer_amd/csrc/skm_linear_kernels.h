@@ -128,8 +128,9 @@ __device__ __forceinline__ float ln_slope(int act, float z)
         return s * (1.0f + z * (1.0f - s));
     }
     case ACT_SIGMOID: {
-        const float s = ln_sigmoid(z);
-        return s * (1.0f - s);
+        // s (1 - s) = e / (1 + e)^2, e = exp(-|z|): 1 - s would keep nothing of itself where s is next to 1 (17 % off at z = 15, 0 from 17 on)
+        const float e = __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
+        return e * r * r;
     }
     default:
         return 1.0f;

@@ -119,3 +119,26 @@ def test_gradients_at_temperatures_near_nothing(ctx, dt, T):
             exact[i, y] += gl[i] / T
             exact[i, s[i].argmax()] -= gl[i] / T
     assert (np.abs(got - exact) <= (4 * U + HALF_STEP[dt] * 1.01) * np.abs(exact)).all()
+
+
+# ---------------------------------------------------------------------------- activations, relative to themselves
+def one_term(ctx, z, name, dt):
+    """(y, slope) of an activation at the values z of type dt, as float64: the product x z with x = 1 is exact, so is the one of dz."""
+    words, zt = rounded(np.asarray(z)[:, None], dt)
+    one = ctx.to_device(rounded(np.ones((1, 1)), dt)[0])
+    y, pre = engine.linear(ctx, ctx.to_device(words), one, activation=name, preact=True)
+    g = ctx.to_device(rounded(np.ones_like(words, dtype=np.float32) if dt != "bf16" else np.ones(words.shape, np.float32), dt)[0])
+    dx, _, _ = engine.linear_backward(ctx, g, None, one, activation=name, preact=pre, dw=None, dbias=None)
+    return zt[:, 0], values(y.download(), dt)[:, 0], values(dx.download(), dt)[:, 0]
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_sigmoids_slope_relative_to_itself(ctx, dt):
+    """e / (1 + e)^2 with e = exp(-|z|): the exponential's argument has one rounding and the instruction's own ulp, (|z| + 2) 2^-23, the rest
+    (the sum, a reciprocal of one ulp twice, two products) below 8 u; half a step of the type follows, of its smallest numbers too."""
+    z, _, got = one_term(ctx, np.concatenate([np.linspace(-80, 80, 641), [12.0, 15.0, 17.0, 20.0]]), "sigmoid", dt)
+    e = np.exp(-np.abs(z))
+    want = e / (1 + e) ** 2
+    room = (np.abs(z) + 2) * 2.0 ** -23 + 8 * U + HALF_STEP[dt] * 1.01
+    assert (np.abs(got - want) <= room * want + SMALLEST[dt]).all()
+    assert (got[np.abs(z) < 10] > 0).all() and np.array_equal(got[:641], got[:641][::-1])  # (an even function)
