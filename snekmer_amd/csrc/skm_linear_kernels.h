@@ -59,18 +59,40 @@ struct ln_type<2> {
     static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c, int) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
-// ---- activations (float32)
-// (exp overflows to inf for z < -88: 0, as it should be; the reciprocal instruction is good to 1 ulp, a rounded division costs ten more)
-__device__ __forceinline__ float ln_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+// ---- activations (in float32)
+// FINE: for float32 outputs, which keep that type's precision however small they are.  16-bit outputs are rounded at 2^-9 or
+// 2^-12 of themselves: the plain exponential, off by |x| u of itself (u = 2^-24: 6e-6 at x = -100), is exact enough for them.
+
+// exp(x + x_lo) for x <= 0 (NaN stays) to 8 u: the rounding of x log2(e) is put back, and the square of exp(x / 2) reaches below
+// 2^-126, where the instruction's own results end
+__device__ __forceinline__ float ln_exp_fine(float x, float x_lo = 0.0f)
+{
+    x = __builtin_elementwise_maximum(x, -110.0f);  // (0 from -104 on)
+    const float t = x * 0.721347511f;               // log2(e) / 2, and what that float leaves out
+    const float lo = __builtin_fmaf(x_lo, 0.721347511f, __builtin_fmaf(x, 9.62981495e-09f, __builtin_fmaf(x, 0.721347511f, -t)));
+    const float h = __builtin_amdgcn_exp2f(t), f = __builtin_fmaf(h, lo * 0.693147181f, h);
+    return f * f;
+}
+
+// (fast: exp overflows to inf for z < -88: 0, as it should be; the reciprocal instruction is good to 1 ulp, a rounded division costs ten more)
+template <bool FINE>
+__device__ __forceinline__ float ln_sigmoid(float z)
+{
+    if (!FINE)
+        return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+    const float e = ln_exp_fine(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
+    return z > 0.0f ? r : e * r;
+}
 
 // The normal distribution's lower tail at -|z|, bell = exp(-z z / 2): tail / (t bell) with t = 1 / (1 + 0.27 |z|) is smooth over all z, a
-// polynomial of degree 8 in t fitted to it (least maximum error over |z| < 14.5) is off by 2.4e-8 of its value.  So gelu keeps its relative precision
-// in the tail, where 1 + erf cancels (4e-6 at z = -12), for one exponential: 4096 x 4096 cells of k = 1024 with residual
-// and pre-activation in 63 us
-// where erff took 74.
+// polynomial of degree 8 in t fitted to it (least maximum error over |z| < 14.5) is off by 3.9e-8 of its value, evaluated in float32
+// by 2.6e-7.  So gelu keeps its relative precision in the tail, where 1 + erf cancels (4e-6 at z = -12), for one exponential: 4096 x
+// 4096 cells of k = 1024 with residual and pre-activation in 63 us where erff took 74 (bfloat16).
+template <bool FINE>
 __device__ __forceinline__ float ln_normal_tail(float z, float &bell)
 {
-    const float a = fabsf(z), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.27f, a, 1.0f));
+    // (FINE: bell is 0 from 15 on; NaN stays)
+    const float a = FINE ? __builtin_elementwise_minimum(fabsf(z), 15.0f) : fabsf(z), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.27f, a, 1.0f));
     float p = 0.0289610978f;
     p = __builtin_fmaf(p, t, -0.126485839f);
     p = __builtin_fmaf(p, t, 0.169786125f);
@@ -80,10 +102,12 @@ __device__ __forceinline__ float ln_normal_tail(float z, float &bell)
     p = __builtin_fmaf(p, t, 0.101810604f);
     p = __builtin_fmaf(p, t, 0.107542872f);
     p = __builtin_fmaf(p, t, 0.107720658f);
-    bell = __expf(-0.5f * a * a);
+    const float q = -0.5f * a * a;
+    bell = FINE ? ln_exp_fine(q, __builtin_fmaf(-0.5f * a, a, -q)) : __expf(q);
     return p * t * bell;
 }
 
+template <bool FINE>
 __device__ __forceinline__ float ln_act(int act, float z)
 {
     switch (act) {
@@ -91,23 +115,24 @@ __device__ __forceinline__ float ln_act(int act, float z)
         return z < 0.0f ? 0.0f : z;  // (NaN stays)
     case ACT_GELU: {
         float bell;
-        const float tail = ln_normal_tail(z, bell);
+        const float tail = ln_normal_tail<FINE>(z, bell);
         return z * (z > 0.0f ? 1.0f - tail : tail);
     }
     case ACT_GELU_TANH: {
         // 0.5 z (1 + tanh u) = z sigmoid(2 u)
         const float u = 0.797884560802865356f * (z + 0.044715f * z * z * z);
-        return z * ln_sigmoid(2.0f * u);
+        return z * ln_sigmoid<FINE>(2.0f * u);
     }
     case ACT_SILU:
-        return z * ln_sigmoid(z);
+        return z * ln_sigmoid<FINE>(z);
     case ACT_SIGMOID:
-        return ln_sigmoid(z);
+        return ln_sigmoid<FINE>(z);
     default:
         return z;
     }
 }
 
+template <bool FINE>
 __device__ __forceinline__ float ln_slope(int act, float z)
 {
     switch (act) {
@@ -115,21 +140,21 @@ __device__ __forceinline__ float ln_slope(int act, float z)
         return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
     case ACT_GELU: {
         float bell;
-        const float tail = ln_normal_tail(z, bell);
+        const float tail = ln_normal_tail<FINE>(z, bell);
         return (z > 0.0f ? 1.0f - tail : tail) + z * bell * 0.398942280401432678f;
     }
     case ACT_GELU_TANH: {
-        const float u2 = 1.59576912160573071f * (z + 0.044715f * z * z * z), s = ln_sigmoid(u2);
-        const float bell = s * (1.0f - s);  // (0 from |z| = 10 on, where z z may be infinite)
+        const float u2 = 1.59576912160573071f * (z + 0.044715f * z * z * z), s = ln_sigmoid<FINE>(u2);
+        const float bell = s * (1.0f - s);  // (0 from |z| = 11 on, where z z may be infinite)
         return bell == 0.0f ? s : s + z * bell * 1.59576912160573071f * (1.0f + 0.134145f * z * z);
     }
     case ACT_SILU: {
-        const float s = ln_sigmoid(z);
+        const float s = ln_sigmoid<FINE>(z);
         return s * (1.0f + z * (1.0f - s));
     }
     case ACT_SIGMOID: {
         // s (1 - s) = e / (1 + e)^2, e = exp(-|z|): 1 - s would keep nothing of itself where s is next to 1 (17 % off at z = 15, 0 from 17 on)
-        const float e = __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
+        const float e = FINE ? ln_exp_fine(-fabsf(z)) : __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
         return e * r * r;
     }
     default:
@@ -203,7 +228,7 @@ __device__ __forceinline__ ln_done<DT, VE> ln_cells(const ln_gemm &g, int act, c
         d.z = ln_pack<DT, VE>(v);
 #pragma unroll
     for (int u = 0; u < VE; ++u)
-        v[u] = ln_act(act, v[u]) + (float)res[u];
+        v[u] = ln_act<DT == 0>(act, v[u]) + (float)res[u];
     d.y = ln_pack<DT, VE>(v);
     return d;
 }
@@ -784,7 +809,7 @@ __global__ __launch_bounds__(NW * 64) void k_linear_few(ln_gemm g)
             v += (float)((const T *)g.bias)[j];
         if (g.preact)
             ((T *)g.preact)[i * g.ldp + j] = (T)v;
-        v = ln_act(g.act, v);
+        v = ln_act<DT == 0>(g.act, v);
         if (g.residual)
             v += (float)((const T *)g.residual)[i * g.ldr + j];
         ((T *)g.out)[i * g.ldo + j] = (T)v;
@@ -905,7 +930,7 @@ __global__ __launch_bounds__(256) void k_linear_dz(int64_t rows, int64_t cols, c
                 for (int u = 0; u < VE; ++u) {
                     float d = (float)v[p][u];
                     if (decltype(ACT)::value != ACT_NONE)
-                        d = r < rows && c + u < cols ? d * ln_slope(decltype(ACT)::value, (float)zz[p][u]) : 0.0f;
+                        d = r < rows && c + u < cols ? d * ln_slope<DT == 0>(decltype(ACT)::value, (float)zz[p][u]) : 0.0f;
                     sum[u] += d;
                     v[p][u] = (T)d;
                 }

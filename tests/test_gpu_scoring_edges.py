@@ -142,3 +142,42 @@ def test_sigmoids_slope_relative_to_itself(ctx, dt):
     room = (np.abs(z) + 2) * 2.0 ** -23 + 8 * U + HALF_STEP[dt] * 1.01
     assert (np.abs(got - want) <= room * want + SMALLEST[dt]).all()
     assert (got[np.abs(z) < 10] > 0).all() and np.array_equal(got[:641], got[:641][::-1])  # (an even function)
+
+
+def test_float32_activations_relative_to_themselves(ctx):
+    """Roundings of float32, u = 2^-24 each.  exp(-|z|): what the argument's rounding loses is put back; the instruction's ulp (2 u) and a
+    rounding, squared, and the square's: 8 u.  sigmoid: 8 + 1 (sum) + 2 (reciprocal) + 1: 16 u covers it.  silu: one more.  gelu: the
+    polynomial 5 u, its argument 3 u, the exponential 8, two products: 32 u.  gelu_tanh: the argument 2 u of the exponential has six
+    roundings, each the argument's size in the result.  Below 2^-126 half a step of the smallest numbers, times z where z multiplies."""
+    z, y, slope = one_term(ctx, np.concatenate([np.linspace(-103, 87, 3801), -(2.0 ** np.arange(-20, 6.5, 0.5))]), "sigmoid", "f32")
+    e = np.exp(-np.abs(z))
+    want = np.where(z > 0, 1 / (1 + e), e / (1 + e))
+    tiny = 2.0 ** -148
+    assert (np.abs(y - want) <= 16 * U * want + tiny).all()
+    want = e / (1 + e) ** 2
+    assert (np.abs(slope - want) <= 20 * U * want + tiny).all()  # (the reciprocal twice)
+    z, y, slope = one_term(ctx, z, "silu", "f32")
+    want = z * np.where(z > 0, 1, e) / (1 + e)
+    assert (np.abs(y - want) <= 17 * U * np.abs(want) + tiny * np.abs(z)).all()
+    low = z < -3  # the slope s (1 + z (1 - s)) has its root at -1.28; here z / (1 + z) is below 1.5
+    s = e / (1 + e)
+    want = (s * (1 + z * (1 - s)))[low]
+    assert (np.abs(slope[low] - want) <= 32 * U * np.abs(want) + tiny * np.abs(z[low])).all()
+    z, y, _ = one_term(ctx, -np.linspace(1e-3, 13.0, 2001), "gelu", "f32")
+    want = z * 0.5 * np.vectorize(math.erfc)(-z / math.sqrt(2.0))
+    assert (np.abs(y - want) <= 32 * U * np.abs(want) + tiny * np.abs(z)).all()
+    z, y, _ = one_term(ctx, np.linspace(-10.2, 10.0, 2001), "gelu_tanh", "f32")
+    two_u = 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+    want = z / (1 + np.exp(-two_u))
+    assert (np.abs(y - want) <= (6 * np.abs(two_u) + 20) * U * np.abs(want) + tiny * np.abs(z)).all()
+
+
+@pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu", "sigmoid"])
+def test_float32_activations_keep_nan_and_reach_their_limits(ctx, name):
+    z, y, slope = one_term(ctx, [np.nan, 300.0, -300.0, 2.0 ** 127, -2.0 ** 127, 0.0, -0.0], name, "f32")
+    assert np.isnan(y[0]) and np.isnan(slope[0])
+    up = np.ones(2) if name == "sigmoid" else z[[1, 3]]
+    assert np.array_equal(y[[1, 3]], up) and np.array_equal(y[[2, 4]], [0, 0])
+    assert np.array_equal(slope[1:5], [0, 0, 0, 0] if name == "sigmoid" else [1, 0, 1, 0])
+    half = 0.5 if name != "sigmoid" else 0.25
+    assert np.allclose(y[5:], 0.5 if name == "sigmoid" else 0.0, rtol=32 * U, atol=0) and np.allclose(slope[5:], half, rtol=32 * U)
