@@ -562,7 +562,8 @@ class Context:
         """Wait for the context's stream.  Errors that only the device can detect are reported HERE (and by downloads), i.e.
         possibly calls later than their cause: a HipError SKM_E_BADARG from sync() / download() naming `max_seq_len` refers
         to an earlier count_csr / vectorize call on this context whose bound was smaller than one of its sequences (those
-        rows were left empty); the word is sticky until reported once."""
+        rows were left empty), one naming a label to an earlier log_probabilities call (those rows are NaN); what was found is kept
+        until it is reported, once, all of it."""
         _check(self.lib, self.lib.skm_sync(self.handle))
 
     # -- HIP graphs (skm_graph_*): record a fixed sequence of calls once, replay it with one launch

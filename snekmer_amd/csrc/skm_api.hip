@@ -332,23 +332,26 @@ extern "C" int skm_stream_wait(skm_ctx *ctx, skm_ctx *src, int slot)
 
 int skm_check_device_error(skm_ctx *ctx, const char *who)
 {
+    static const char *const TEXT[SKM_DEVERR_COUNT] = {
+        "an earlier skm_count_csr / skm_vectorize_csr call on this context was given a max_seq_len smaller than one of its sequences; the rows "
+        "of those sequences were left EMPTY (pass 0 or a true bound)",
+        "an earlier skm_log_probabilities / skm_log_probabilities_backward call on this context was given a label outside [-1, cols); those "
+        "rows' log probabilities and gradients were set to NaN",
+    };
     volatile uint32_t *w = (volatile uint32_t *)ctx->h_pinned + SKM_DEVERR_WORD;
-    const uint32_t bits = *w;
-    if (!bits)
+    std::string all;
+    for (int i = 0; i < SKM_DEVERR_COUNT; ++i) {
+        if (!w[i])
+            continue;
+        w[i] = 0;
+        if (!all.empty())
+            all += "; ";
+        all += TEXT[i];
+    }
+    if (all.empty())
         return SKM_OK;
-    *w = 0;
-    if (bits & SKM_DEVERR_SEQ_TOO_LONG) {
-        skm_set_error("%s: an earlier skm_count_csr / skm_vectorize_csr call on this context was given a max_seq_len smaller than "
-                      "one of its sequences; the rows of those sequences were left EMPTY (pass 0 or a true bound)", who);
-        return SKM_E_BADARG;
-    }
-    if (bits & SKM_DEVERR_LABEL) {
-        skm_set_error("%s: an earlier skm_log_probabilities / skm_log_probabilities_backward call on this context was given a label outside "
-                      "[-1, cols); those rows' log probabilities and gradients were set to NaN", who);
-        return SKM_E_BADARG;
-    }
-    skm_set_error("%s: a kernel reported error bits 0x%x", who, bits);
-    return SKM_E_HIP;
+    skm_set_error("%s: %s", who, all.c_str());
+    return SKM_E_BADARG;
 }
 
 extern "C" int skm_sync(skm_ctx *ctx)

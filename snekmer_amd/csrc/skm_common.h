@@ -47,9 +47,11 @@ struct skm_ctx {
     void *ws[WS_COUNT] = {};
     size_t ws_bytes[WS_COUNT] = {};
     void *h_pinned = nullptr;  // small pinned buffer for count read-backs
-    // Sticky device-side error word: word SKM_DEVERR_WORD of h_pinned, written by kernels through its device address when an
-    // argument the host cannot check turns out wrong on the device (a sequence longer than the caller's max_seq_len); read
-    // and cleared by skm_check_device_error wherever the library has just waited for the stream.  nullptr: not addressable.
+    // Sticky device-side error words: words SKM_DEVERR_WORD + skm_deverr of h_pinned, written by kernels (see skm_err_word)
+    // when an argument the host cannot check turns out wrong on the device (a sequence longer than the caller's max_seq_len);
+    // read and cleared by skm_check_device_error wherever the library has just waited for the stream.  A word an error: kernels
+    // store 1 (to set a bit among others they would have to read and write host memory, which needs PCIe atomics).  This is
+    // their first word's device address; nullptr: not addressable.
     uint32_t *d_err = nullptr;
     hipEvent_t ev_host = nullptr;  // marks an asynchronous read-back the host waits for while later kernels run
     bool profiling = false;
@@ -98,9 +100,10 @@ void skm_pinned_release(int device, void *page);
 bool skm_foreign_capture(const skm_ctx *ctx);
 void skm_graph_release(struct skm_graph *graph);
 constexpr int SKM_DEVERR_WORD = 768;  // byte 3072 of h_pinned
-constexpr uint32_t SKM_DEVERR_SEQ_TOO_LONG = 1u;
-constexpr uint32_t SKM_DEVERR_LABEL = 2u;
-// Call after a stream synchronise: reports (once) what kernels flagged since the last check.
+enum skm_deverr { SKM_DEVERR_SEQ_TOO_LONG = 0, SKM_DEVERR_LABEL, SKM_DEVERR_COUNT };
+// the word that a kernel sets to 1 to report `what` (nullptr: it cannot)
+static inline uint32_t *skm_err_word(const skm_ctx *ctx, skm_deverr what) { return ctx->d_err ? ctx->d_err + what : nullptr; }
+// Call after a stream synchronise: reports (once) everything that kernels flagged since the last check.
 int skm_check_device_error(skm_ctx *ctx, const char *who);
 // similarity -> distance in place over a float32 block: out = clamp(1 - out, 0, 2), no diagonal rule (the epilogue of
 // mode 2 of skm_cosine_csr / skm_cosine_dense_i8: sklearn's cosine_distances(X, Y) with Y another matrix than X);

@@ -79,10 +79,10 @@ __global__ void k_classify(const uint8_t *__restrict__ seq, const int64_t *__res
         w = 0;
     if (max_win >= 0 && w > max_win) {
         // longer than the bound the caller gave (which sized the launches and the scratch behind this kernel): the row
-        // stays empty and the context's sticky error word says so at the next host wait (skm_check_device_error)
+        // stays empty and the context's sticky error word for it says so at the next host wait (skm_check_device_error)
         w = 0;
-        if (err)  // one bit is defined: a plain system-scope store (a read-modify-write on host memory needs PCIe atomics)
-            __hip_atomic_store(err, SKM_DEVERR_SEQ_TOO_LONG, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        if (err)
+            __hip_atomic_store(err, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     }
     if (slen)
         slen[i] = (int32_t)len;
@@ -820,7 +820,7 @@ int count_csr_impl(skm_ctx *ctx, const skm_lut256 &lut, int nsym, int k, const u
         SKM_PROF(ctx, "k_classify");
         const int64_t max_win = max_seq_len > 0 ? (max_seq_len - k + 1 > 0 ? max_seq_len - k + 1 : 0) : -1;
         k_classify<<<(unsigned)skm_ceil_div(n, 256), 256, 0, st>>>(d_seq, d_off, n, k, slen, nullptr, lists, fill,
-                                                                     row_nnz, max_win, ctx->d_err);
+                                                                     row_nnz, max_win, skm_err_word(ctx, SKM_DEVERR_SEQ_TOO_LONG));
     }
     SKM_TRY(skm_check_launch("k_classify"));
     // Every count kernel reads its list length on the device and is launched with a grid that covers the worst case,

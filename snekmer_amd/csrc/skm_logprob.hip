@@ -583,7 +583,7 @@ __device__ __forceinline__ void lp_finish(int64_t row0, int nrows, float m, floa
             if (y < -1 || y >= a.cols) {
                 v = nan;
                 if (a.err)
-                    __hip_atomic_store(a.err, SKM_DEVERR_LABEL, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+                    __hip_atomic_store(a.err, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
             } else if (y >= 0) {
                 if (bad) {
                     v = nan;
@@ -794,7 +794,7 @@ __global__ __launch_bounds__(256) void k_log_probabilities_grad(lp_grad_args a)
         const int64_t y = !a.d_logp ? -1 : a.label64 ? ((const int64_t *)a.labels)[row] : (int64_t)((const int32_t *)a.labels)[row];
         const bool wrong = y < -1 || y >= a.cols;
         if (wrong && a.err && lane == 0)
-            __hip_atomic_store(a.err, SKM_DEVERR_LABEL, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            __hip_atomic_store(a.err, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         const float gl = wrong ? __builtin_nanf("") : y >= 0 ? a.d_logp[row] : 0.0f;
         const float gh = a.d_entropy ? a.d_entropy[row] : 0.0f;
         const float m = a.stats[2 * row], l = a.stats[2 * row + 1], hl = (a.d_entropy ? a.entropy[row] : 0.0f) - l;
@@ -976,7 +976,7 @@ extern "C" int skm_log_probabilities(skm_ctx *ctx, int dtype, int64_t rows, int6
     a.stats = d_stats;
     a.top_index = d_top_index;
     a.top_logp = d_top_logp;
-    a.err = ctx->d_err;
+    a.err = skm_err_word(ctx, SKM_DEVERR_LABEL);
     const lp_cut cut = lp_plan(ctx, rows, cols);
     a.nsplit = cut.nsplit;
     a.tiles_per_split = cut.tiles_per_split;
@@ -1043,7 +1043,7 @@ extern "C" int skm_log_probabilities_backward(skm_ctx *ctx, int dtype, int64_t r
     a.d_entropy = d_grad_entropy;
     a.out = d_grad_scores;
     a.ldo = ldg;
-    a.err = ctx->d_err;
+    a.err = skm_err_word(ctx, SKM_DEVERR_LABEL);
     const int64_t units = rows * skm_ceil_div(cols, LP_TILE);
     const unsigned grid = (unsigned)std::min<int64_t>((int64_t)1 << 23, skm_ceil_div(units, 4));
     SKM_PROF(ctx, "k_log_probabilities_grad");

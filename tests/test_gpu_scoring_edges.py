@@ -181,3 +181,25 @@ def test_float32_activations_keep_nan_and_reach_their_limits(ctx, name):
     assert np.array_equal(slope[1:5], [0, 0, 0, 0] if name == "sigmoid" else [1, 0, 1, 0])
     half = 0.5 if name != "sigmoid" else 0.25
     assert np.allclose(y[5:], 0.5 if name == "sigmoid" else 0.0, rtol=32 * U, atol=0) and np.allclose(slope[5:], half, rtol=32 * U)
+
+
+# ---------------------------------------------------------------------------- errors that only the device sees
+@pytest.mark.parametrize("first", ["sequence", "label"])
+def test_two_errors_at_once_are_both_reported(ctx, first):
+    """A bound that a sequence exceeds and a label that is no class, neither waited for in between: one report names both, once."""
+    from snekmer_amd import alphabet
+
+    own = _hip.Context(0)
+    lut = alphabet.build_lut("hydro")
+    batch = engine.SeqBatch.from_strings(own, ["MKVLAAGIWMKVLAAGIW", "MKVL"])
+    batch.max_len = 6
+    s = own.to_device(whole_numbers((3, 20), 1))
+    labels = own.to_device(np.array([0, 20, 1], np.int32))
+    calls = [lambda: engine.vectorize_fused(own, batch, lut, 4), lambda: apply.log_probabilities(own, s, labels)]
+    kept = [call() for call in (calls if first == "sequence" else calls[::-1])]
+    with pytest.raises(_hip.HipError, match="EMPTY") as e:
+        own.sync()
+    assert e.value.code == -1 and "label outside" in str(e.value)
+    own.sync()
+    del kept
+    own.close()
