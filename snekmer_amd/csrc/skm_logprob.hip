@@ -917,6 +917,20 @@ struct lp_span {
 };
 bool lp_share(const lp_span &a, const lp_span &b) { return skm_overlap(a.p, a.rows, a.bytes, a.stride, b.p, b.rows, b.bytes, b.stride, 1); }
 
+// float32 and integer arrays are read and written as such
+struct lp_vector {
+    const char *what;
+    const void *p;
+    int bytes;
+};
+template <int N>
+int lp_check_aligned(const char *who, const lp_vector (&vectors)[N])
+{
+    for (const lp_vector &v : vectors)
+        SKM_REQUIRE((uintptr_t)v.p % (uintptr_t)v.bytes == 0, SKM_E_BADARG, "%s: %s is not aligned to its type", who, v.what);
+    return SKM_OK;
+}
+
 // what both entry points check
 int lp_check(const char *who, skm_ctx *ctx, int dtype, int64_t rows, int64_t cols, const void *d_scores, int64_t ld, const uint8_t *d_mask, int64_t ldmask,
              int label_bits, double temperature)
@@ -949,6 +963,7 @@ extern "C" int skm_log_probabilities(skm_ctx *ctx, int dtype, int64_t rows, int6
     SKM_REQUIRE(!d_logp || d_labels || rows == 0, SKM_E_BADARG, "%s: log probabilities need labels", who);
     if (rows == 0)
         return SKM_OK;
+    SKM_TRY(lp_check_aligned(who, {{"labels", d_labels, label_bits / 8}, {"logp", d_logp, 4}, {"entropy", d_entropy, 4}, {"stats", d_stats, 4}, {"top_index", d_top_index, 4}, {"top_logp", d_top_logp, 4}}));
     const int64_t es = dtype == 0 ? 4 : 2;
     const lp_span in[3] = {{d_scores, rows, cols * es, ld * es}, {d_mask, ldmask ? rows : 1, cols, ldmask ? ldmask : cols}, {d_logp ? d_labels : nullptr, 1, rows * (label_bits / 8), rows * (label_bits / 8)}};
     const lp_span out[5] = {{d_logp, 1, rows * 4, rows * 4}, {d_entropy, 1, rows * 4, rows * 4}, {d_stats, 1, rows * 8, rows * 8}, {d_top_index, 1, rows * k * 4, rows * k * 4}, {d_top_logp, 1, rows * k * 4, rows * k * 4}};
@@ -1016,6 +1031,7 @@ extern "C" int skm_log_probabilities_backward(skm_ctx *ctx, int dtype, int64_t r
         return SKM_OK;
     SKM_REQUIRE(d_stats && d_grad_scores && (!d_grad_logp || d_labels) && (!d_grad_entropy || d_entropy), SKM_E_BADARG,
                 "%s: null array (stats, the output, labels for grad_logp, entropy for grad_entropy)", who);
+    SKM_TRY(lp_check_aligned(who, {{"labels", d_labels, label_bits / 8}, {"stats", d_stats, 4}, {"entropy", d_entropy, 4}, {"grad_logp", d_grad_logp, 4}, {"grad_entropy", d_grad_entropy, 4}}));
     SKM_REQUIRE(((uintptr_t)d_grad_scores & (dtype == 0 ? 3 : 1)) == 0, SKM_E_BADARG, "%s: the output is not aligned to its type", who);
     const int64_t es = dtype == 0 ? 4 : 2;
     SKM_REQUIRE((d_grad_scores == d_scores && ldg == ld) || !skm_overlap(d_grad_scores, rows, cols, ldg, d_scores, rows, cols, ld, es), SKM_E_BADARG,

@@ -203,3 +203,42 @@ def test_two_errors_at_once_are_both_reported(ctx, first):
     own.sync()
     del kept
     own.close()
+
+
+class At:
+    """An array of another library at any address."""
+
+    def __init__(self, base, shape, typestr, offset):
+        self.base, self.shape = base, shape
+        self.interface = {"shape": shape, "typestr": typestr, "data": (base.ptr + offset, False), "strides": None, "version": 2}
+
+    @property
+    def __cuda_array_interface__(self):
+        return self.interface
+
+
+def test_vectors_between_addresses_of_their_type_are_refused(ctx):
+    """The rows' vectors are read and written as whole elements (scores, as documented, need no more than their own type's alignment)."""
+    s = ctx.to_device(whole_numbers((4, 10), 1))
+    room = ctx.zeros(400, np.uint8)
+    labels = ctx.to_device(np.arange(4, dtype=np.int32))
+    fwd = apply.log_probabilities(ctx, s, labels)
+    ones = ctx.to_device(np.ones(4, np.float32))
+    f, i = "<f4", "<i4"
+    for name, out in (("logp", At(room, (4,), f, 2)), ("entropy", At(room, (4,), f, 1)), ("stats", At(room, (4, 2), f, 6)), ("top_index", At(room, (4, 2), i, 2)),
+                      ("top_logp", At(room, (4, 2), f, 3))):
+        with pytest.raises(_hip.HipError, match=f"{name} is not aligned"):
+            apply.log_probabilities(ctx, s, labels, k=2, out=apply.LogProbabilities(**{name: out}))
+    for wrong in (At(room, (4,), i, 2), At(room, (4,), "<i8", 4)):
+        with pytest.raises(_hip.HipError, match="labels is not aligned"):
+            apply.log_probabilities(ctx, s, wrong)
+    backward = lambda **more: apply.log_probabilities_backward(ctx, s, more.pop("labels", labels), more.pop("forward", fwd), **more)
+    for name, call in (("labels", lambda: backward(labels=At(room, (4,), "<i8", 4), d_logp=ones)), ("grad_logp", lambda: backward(d_logp=At(room, (4,), f, 2))),
+                       ("grad_entropy", lambda: backward(d_entropy=At(room, (4,), f, 2))),
+                       ("stats", lambda: backward(d_logp=ones, forward=apply.LogProbabilities(stats=At(room, (4, 2), f, 2)))),
+                       ("entropy", lambda: backward(d_entropy=ones, forward=apply.LogProbabilities(stats=fwd.stats, entropy=At(room, (4,), f, 2))))):
+        with pytest.raises(_hip.HipError, match=f"{name} is not aligned"):
+            call()
+    four = apply.log_probabilities(ctx, s, At(room, (4,), "<i8", 8), out=apply.LogProbabilities(logp=At(room, (4,), f, 100), stats=At(room, (4, 2), f, 204)))
+    ctx.sync()
+    assert four.host() == {}  # (on their own addresses they are taken)
