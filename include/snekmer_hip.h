@@ -388,7 +388,7 @@ int skm_row_top2(skm_ctx *ctx, int64_t n, int64_t m, const float *d_scores, int6
  *   d_scores [rows x cols], row stride ld >= cols elements of any alignment; dtype 0 float32, 1 float16, 2 bfloat16
  *   d_mask   NULL, or bytes: 0 where a class may not be chosen; row stride ldmask >= cols, 0: one row for all
  *   d_labels the given class of each row (label_bits 32 or 64, signed), -1: none
- *   p = softmax(scores / temperature) over the allowed classes: mask != 0 and score > -infinity
+ *   p = softmax(scores / temperature) over the allowed classes: mask != 0 and score > -infinity; 1e-30 < temperature < 1e30
  * Outputs (float32 / int32, like the labels on addresses of their type; each may be NULL):
  *   d_logp[rows]        log p(label); 0 for label -1; -infinity where the label is not allowed
  *   d_entropy[rows]     in nats

@@ -167,8 +167,8 @@ def _score_arguments(ctx, scores, labels, mask, ncols, temperature):
         cols = int(ncols)
     if cols < 1:
         raise ValueError("scores: no classes")
-    if not 0.0 < float(temperature) < float("inf"):
-        raise ValueError(f"temperature: {temperature} (want a positive number)")
+    if not 1e-30 < float(temperature) < 1e30:  # (what the library takes: 1 / T and log2(e) / T stay ordinary float32 numbers)
+        raise ValueError(f"temperature: {temperature} (want a positive number between 1e-30 and 1e30)")
     mp, ldmask = None, 0
     if mask is not None:
         two = len(getattr(mask, "shape", ())) == 2
@@ -212,7 +212,7 @@ def log_probabilities(ctx, scores, labels=None, k: int = 0, temperature: float =
     `scores` [n, ld] float32, float16 or `_hip.bfloat16`, of which the first `ncols` columns count (default: all); `labels` [n]:
     class ids on the device (int32 / int64) or on the host, -1 where none is known (log probability 0); `mask`: uint8 or bool
     on the device, 0 where a class may not be chosen, [ncols] for all rows or [n, ncols]; a score of -infinity is a class that
-    may not be chosen either.  `k` <= 16 alternatives, padded with (-1, -inf).  A row that allows nothing has entropy 0 and
+    may not be chosen either.  `temperature`: between 1e-30 and 1e30.  `k` <= 16 alternatives, padded with (-1, -inf).  A row that allows nothing has entropy 0 and
     log probability -inf; one that allows a NaN or +inf is NaN throughout, with indices -1.  A label on the device outside
     [-1, ncols) gives NaN and is reported by the next Context.sync / download.  `out`: a LogProbabilities whose members are
     filled (arrays of this library or of another one); only those it has are computed."""

@@ -6,6 +6,9 @@ import subprocess
 
 import pytest
 
+from snekmer_amd import _hip, apply, engine
+from test_scoring import CTX, LABELS, Fake, NoDevice, S, _stats
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "snekmer_amd", "csrc")
 
@@ -57,3 +60,12 @@ int main()
 }
 """)
     assert int(out.split()[-1]) > 100000
+
+
+@pytest.mark.parametrize("T", [1e-31, 1e-30, 1e30, 1e31, -1.0])
+def test_temperatures_that_the_library_does_not_take(T):
+    """Both layers refuse the same ones; the Python layer says so as it says it of any other argument."""
+    for call in (lambda: apply.log_probabilities(CTX, S, LABELS, temperature=T),
+                 lambda: apply.log_probabilities_backward(CTX, S, LABELS, _stats(), d_logp=Fake((4,)), temperature=T)):
+        with pytest.raises(ValueError, match="temperature.*between"):
+            call()
