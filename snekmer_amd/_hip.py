@@ -371,7 +371,8 @@ def float_dtype(code: int) -> np.dtype:
 
 
 def is_device_array(x) -> bool:
-    return isinstance(x, DeviceArray) or hasattr(type(x), "__cuda_array_interface__")
+    # (torch's tensors all have the interface by type; on the host there is only an error behind it)
+    return isinstance(x, DeviceArray) or (hasattr(type(x), "__cuda_array_interface__") and getattr(x, "is_cuda", True))
 
 
 _TENSOR_TYPES = {}  # type string by dtype object, of arrays that also answer data_ptr() / stride() (see array_view)

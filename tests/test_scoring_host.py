@@ -69,3 +69,41 @@ def test_temperatures_that_the_library_does_not_take(T):
                  lambda: apply.log_probabilities_backward(CTX, S, LABELS, _stats(), d_logp=Fake((4,)), temperature=T)):
         with pytest.raises(ValueError, match="temperature.*between"):
             call()
+
+
+class HostTensor:
+    """A tensor of a library whose type has the array interface, on the host: an error is behind it."""
+
+    is_cuda = False
+
+    def __init__(self, values):
+        self.values = values
+
+    @property
+    def __cuda_array_interface__(self):
+        raise AttributeError("the tensor is on the host")
+
+    def __array__(self, dtype=None, copy=None):
+        import numpy as np
+
+        return np.asarray(self.values, dtype=dtype)
+
+
+def test_labels_in_another_librarys_host_memory():
+    """Labels may lie on the host, in whatever reads as an array there; they are looked at and copied like a list."""
+    uploads, calls = [], []
+
+    class Recorder(NoDevice):
+        def to_device(self, host):
+            uploads.append(host.tolist())
+            return Fake(host.shape, "<i4")
+
+        def call(self, name, *args):
+            calls.append(name)
+
+    apply.log_probabilities(Recorder(), S, HostTensor([0, 5, -1, 2]))
+    assert uploads == [[0, 5, -1, 2]] and calls == ["skm_log_probabilities"]
+    with pytest.raises(ValueError, match="labels: outside"):
+        apply.log_probabilities(Recorder(), S, HostTensor([0, 6, -1, 2]))
+    with pytest.raises(TypeError, match="on the device"):  # scores may not
+        apply.log_probabilities(Recorder(), HostTensor([[1.0, 2.0]]), [0])
