@@ -60,7 +60,8 @@ extern "C" int skm_linear_backward(skm_ctx *ctx, int dtype, int activation, int6
     SKM_REQUIRE(dtype >= 0 && dtype <= 2, SKM_E_BADARG, "%s: dtype must be 0 (float32), 1 (float16) or 2 (bfloat16)", who);
     SKM_REQUIRE(activation >= 0 && activation < ACT_COUNT, SKM_E_BADARG, "%s: unknown activation %d", who, activation);
     SKM_REQUIRE(m >= 0 && n >= 0 && k >= 0, SKM_E_BADARG, "%s: negative size", who);
-    SKM_REQUIRE(d_dx || d_dw || d_dbias || (m == 0 && n == 0), SKM_E_BADARG, "%s: no gradient is asked for", who);
+    // (a gradient without cells may have no address)
+    SKM_REQUIRE(d_dx || d_dw || d_dbias || m == 0 || n == 0 || k == 0, SKM_E_BADARG, "%s: no gradient is asked for", who);
     const int64_t es = (int64_t)elem_bytes(dtype);
     const bool cells = m > 0 && n > 0;
     SKM_REQUIRE(!cells || d_dy, SKM_E_BADARG, "%s: null dy", who);

@@ -1026,9 +1026,9 @@ extern "C" int skm_log_probabilities_backward(skm_ctx *ctx, int dtype, int64_t r
     const char *who = "skm_log_probabilities_backward";
     SKM_TRY(lp_check(who, ctx, dtype, rows, cols, d_scores, ld, d_mask, ldmask, label_bits, temperature));
     SKM_REQUIRE(ldg >= cols, SKM_E_BADARG, "%s: ldg (%lld) < cols (%lld)", who, (long long)ldg, (long long)cols);
-    SKM_REQUIRE(d_grad_logp || d_grad_entropy, SKM_E_BADARG, "%s: neither a gradient of the log probabilities nor one of the entropies", who);
     if (rows == 0)
         return SKM_OK;
+    SKM_REQUIRE(d_grad_logp || d_grad_entropy, SKM_E_BADARG, "%s: neither a gradient of the log probabilities nor one of the entropies", who);
     SKM_REQUIRE(d_stats && d_grad_scores && (!d_grad_logp || d_labels) && (!d_grad_entropy || d_entropy), SKM_E_BADARG,
                 "%s: null array (stats, the output, labels for grad_logp, entropy for grad_entropy)", who);
     SKM_TRY(lp_check_aligned(who, {{"labels", d_labels, label_bits / 8}, {"stats", d_stats, 4}, {"entropy", d_entropy, 4}, {"grad_logp", d_grad_logp, 4}, {"grad_entropy", d_grad_entropy, 4}}));

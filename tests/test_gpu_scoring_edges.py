@@ -242,3 +242,45 @@ def test_vectors_between_addresses_of_their_type_are_refused(ctx):
     four = apply.log_probabilities(ctx, s, At(room, (4,), "<i8", 8), out=apply.LogProbabilities(logp=At(room, (4,), f, 100), stats=At(room, (4, 2), f, 204)))
     ctx.sync()
     assert four.host() == {}  # (on their own addresses they are taken)
+
+
+# ---------------------------------------------------------------------------- arrays without cells
+class Nowhere:
+    """An array without cells, as other libraries hold it: at address 0."""
+
+    def __init__(self, shape, typestr="<f4"):
+        assert 0 in shape
+        self.shape = shape
+        self.interface = {"shape": shape, "typestr": typestr, "data": (0, False), "strides": None, "version": 2}
+
+    @property
+    def __cuda_array_interface__(self):
+        return self.interface
+
+
+def test_arrays_without_cells_need_no_address(ctx):
+    f = np.float32
+    w, x = ctx.to_device(whole_numbers((4, 5), 1)), ctx.to_device(whole_numbers((3, 5), 2))
+    engine.linear(ctx, Nowhere((0, 5)), w, residual=Nowhere((0, 4)), preact=Nowhere((0, 4)), out=Nowhere((0, 4)))
+    y = engine.linear(ctx, Nowhere((3, 0)), Nowhere((4, 0)), bias=ctx.to_device(np.ones(4, f)))
+    assert (y.download() == 1).all()
+    # no rows: dx has no cells, dw and dbias are empty sums
+    dx = Nowhere((0, 5))
+    assert engine.linear_backward(ctx, Nowhere((0, 4)), None, w, dx=dx, dw=None, dbias=None)[0] is dx
+    _, dw, db = engine.linear_backward(ctx, Nowhere((0, 4)), Nowhere((0, 5)), w, dx=dx)
+    assert (dw.download() == 0).all() and (db.download() == 0).all()
+    # no outputs, no features
+    dx, dw, db = engine.linear_backward(ctx, Nowhere((3, 0)), x, Nowhere((0, 5)), dw=Nowhere((0, 5)), dbias=Nowhere((0,)))
+    assert (dx.download() == 0).all()
+    engine.linear_backward(ctx, ctx.to_device(whole_numbers((3, 4), 3)), Nowhere((3, 0)), Nowhere((4, 0)), dx=Nowhere((3, 0)), dw=Nowhere((4, 0)), dbias=None)
+    _, _, db = engine.linear_backward(ctx, ctx.to_device(np.ones((3, 4), f)), Nowhere((3, 0)), Nowhere((4, 0)), dx=Nowhere((3, 0)), dw=Nowhere((4, 0)))
+    assert (db.download() == 3).all()
+    # no score rows
+    s, one = Nowhere((0, 7)), Nowhere((0,))
+    out = apply.LogProbabilities(logp=one, entropy=Nowhere((0,)), stats=Nowhere((0, 2)), top_index=Nowhere((0, 3), "<i4"), top_logp=Nowhere((0, 3)))
+    apply.log_probabilities(ctx, s, Nowhere((0,), "<i8"), k=3, out=out)
+    for more in (dict(d_logp=one), dict(d_entropy=one), dict(d_logp=one, d_entropy=one)):
+        apply.log_probabilities_backward(ctx, s, Nowhere((0,), "<i4"), out, out=s, **more)
+    with pytest.raises(_hip.HipError, match="no gradient is asked for"):
+        engine.linear_backward(ctx, ctx.to_device(whole_numbers((3, 4), 3)), x, w, dx=None, dw=None, dbias=None)
+    ctx.sync()
