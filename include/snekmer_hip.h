@@ -397,7 +397,8 @@ int skm_row_top2(skm_ctx *ctx, int64_t n, int64_t m, const float *d_scores, int6
  *   d_top_index, d_top_logp [rows x k], 0 <= k <= 16: the best classes, larger scores first, lower indices first among
  *                       equal scores; -1 and -infinity behind the last allowed class
  * A row without an allowed class: stats -infinity, logp -infinity, entropy 0.  A row that allows a NaN or +infinity has
- * no distribution: NaN everywhere, indices -1.  A label outside [-1, cols) gives NaN, and the next skm_sync reports it.
+ * no distribution: NaN everywhere, indices -1.  A label outside [-1, cols) gives NaN, and the next skm_sync reports it (a
+ * replay of a graph that the owner of the context's stream captured only gives NaN).
  * Differences of scores are taken before the temperature divides, the sums are float32, and S + 1 is never formed where
  * one class holds nearly all of the mass (log1p).  Few long rows take scratch memory.  Outputs that share memory with an input or
  * with each other are refused. */

@@ -101,8 +101,9 @@ bool skm_foreign_capture(const skm_ctx *ctx);
 void skm_graph_release(struct skm_graph *graph);
 constexpr int SKM_DEVERR_WORD = 768;  // byte 3072 of h_pinned
 enum skm_deverr { SKM_DEVERR_SEQ_TOO_LONG = 0, SKM_DEVERR_LABEL, SKM_DEVERR_COUNT };
-// the word that a kernel sets to 1 to report `what` (nullptr: it cannot)
-static inline uint32_t *skm_err_word(const skm_ctx *ctx, skm_deverr what) { return ctx->d_err ? ctx->d_err + what : nullptr; }
+// The word that a kernel sets to 1 to report `what`; nullptr: it cannot, or the owner of the context's stream captures the call -
+// its graph may be replayed when the context and its page are gone or another context's.
+static inline uint32_t *skm_err_word(const skm_ctx *ctx, skm_deverr what) { return ctx->d_err && !skm_foreign_capture(ctx) ? ctx->d_err + what : nullptr; }
 // Call after a stream synchronise: reports (once) everything that kernels flagged since the last check.
 int skm_check_device_error(skm_ctx *ctx, const char *who);
 // similarity -> distance in place over a float32 block: out = clamp(1 - out, 0, 2), no diagonal rule (the epilogue of

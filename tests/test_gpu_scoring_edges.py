@@ -284,3 +284,10 @@ def test_arrays_without_cells_need_no_address(ctx):
     with pytest.raises(_hip.HipError, match="no gradient is asked for"):
         engine.linear_backward(ctx, ctx.to_device(whole_numbers((3, 4), 3)), x, w, dx=None, dw=None, dbias=None)
     ctx.sync()
+
+
+# ---------------------------------------------------------------------------- beside other libraries
+def test_while_torch_captures():
+    """tests/torch_interop_edges.py, in a process that loads torch first."""
+    run = subprocess.run([sys.executable, "-u", os.path.join(os.path.dirname(__file__), "torch_interop_edges.py")], capture_output=True, text=True, timeout=110)
+    assert run.returncode == 0 and run.stdout.rstrip().endswith("all passed"), run.stdout + run.stderr

@@ -1,0 +1,74 @@
+"""Contexts over torch's streams while torch captures them.  Run as a program (tests/test_gpu_scoring_edges.py does): torch has to be
+loaded before the library, so that both use one HIP runtime."""
+import os
+import sys
+
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+import numpy as np  # noqa: E402
+
+from snekmer_amd import _hip, apply, engine  # noqa: E402
+
+
+def raises(kind, says, call):
+    try:
+        call()
+    except kind as e:
+        assert says in str(e), e
+        return
+    raise AssertionError(f"{says}: nothing was raised")
+
+
+def a_graph_that_outlives_its_context():
+    """Forward and backward captured by torch; the context goes, another takes over what it held; replays give NaN for wrong labels and
+    report nothing to the other context, and what they compute is what eager calls give."""
+    s = torch.cuda.Stream()
+    own = _hip.Context(0, stream=s.cuda_stream)
+    n, a = 40, 300
+    with torch.cuda.stream(s):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(2)
+        scores = torch.randn(n, a, generator=g, device="cuda")
+        labels = torch.randint(0, a, (n,), generator=g, device="cuda", dtype=torch.int32)
+        d_logp = torch.randn(n, generator=g, device="cuda")
+        logp, entropy = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+        stats, grad = torch.empty(n, 2, device="cuda"), torch.empty(n, a, device="cuda")
+        out = apply.LogProbabilities(logp=logp, entropy=entropy, stats=stats)
+
+        def step(ctx):
+            apply.log_probabilities(ctx, scores, labels, out=out)
+            apply.log_probabilities_backward(ctx, scores, labels, out, d_logp=d_logp, out=grad)
+
+        step(own)
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            step(own)
+        own.sync()
+        own.close()
+        other = _hip.Context(0, stream=s.cuda_stream)
+        for wrong in (a, -7, a + 1, 5):
+            labels[3] = wrong
+            logp.zero_()
+            grad.zero_()
+            graph.replay()
+            other.sync()
+            replayed = [logp.clone(), grad.clone()]
+            bad = wrong != 5
+            assert bool(torch.isnan(logp[3])) == bad and bool(torch.isnan(grad[3]).all()) == bad
+            assert bool(torch.isfinite(logp[4:]).all()) and bool(torch.isfinite(grad[:3]).all())
+            step(other)
+            if bad:
+                raises(_hip.HipError, "label outside", other.sync)  # (an eager call still says so)
+            for x, y in zip(replayed, (logp, grad)):
+                assert torch.equal(torch.nan_to_num(x, 7.0), torch.nan_to_num(y, 7.0))
+        other.sync()
+        other.close()
+
+
+for check in (a_graph_that_outlives_its_context,):
+    print(check.__name__, flush=True)
+    check()
+print("all passed", flush=True)
