@@ -357,6 +357,7 @@ int skm_check_device_error(skm_ctx *ctx, const char *who)
 extern "C" int skm_sync(skm_ctx *ctx)
 {
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     return skm_check_device_error(ctx, "skm_sync");
 }
@@ -436,6 +437,7 @@ extern "C" int skm_memcpy_h2d(skm_ctx *ctx, void *d_dst, const void *h_src, size
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     if (!bytes)
         return SKM_OK;
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipMemcpyAsync(d_dst, h_src, bytes, hipMemcpyHostToDevice, ctx->stream));
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     return SKM_OK;
@@ -447,6 +449,7 @@ extern "C" int skm_memcpy_h2d_async(skm_ctx *ctx, void *d_dst, const void *h_src
     if (!bytes)
         return SKM_OK;
     SKM_REQUIRE(d_dst && h_src_pinned, SKM_E_BADARG, "skm_memcpy_h2d_async: null array");
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipMemcpyAsync(d_dst, h_src_pinned, bytes, hipMemcpyHostToDevice, ctx->stream));
     return SKM_OK;
 }
@@ -456,6 +459,7 @@ extern "C" int skm_memcpy_d2h(skm_ctx *ctx, void *h_dst, const void *d_src, size
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     if (!bytes)
         return SKM_OK;
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipMemcpyAsync(h_dst, d_src, bytes, hipMemcpyDeviceToHost, ctx->stream));
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     return skm_check_device_error(ctx, "skm_memcpy_d2h");
@@ -466,6 +470,7 @@ extern "C" int skm_memcpy_d2d(skm_ctx *ctx, void *d_dst, const void *d_src, size
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     if (!bytes)
         return SKM_OK;
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipMemcpyAsync(d_dst, d_src, bytes, hipMemcpyDeviceToDevice, ctx->stream));
     return SKM_OK;
 }
@@ -475,6 +480,7 @@ extern "C" int skm_memset(skm_ctx *ctx, void *d_dst, int byte_value, size_t byte
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     if (!bytes)
         return SKM_OK;
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipMemsetAsync(d_dst, byte_value, bytes, ctx->stream));
     return SKM_OK;
 }
@@ -654,6 +660,7 @@ extern "C" int skm_profile_enable(skm_ctx *ctx, int on)
 extern "C" int skm_profile_reset(skm_ctx *ctx)
 {
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     for (auto &p : ctx->prof) {
         ctx->event_pool.push_back(p.start);
@@ -666,6 +673,7 @@ extern "C" int skm_profile_reset(skm_ctx *ctx)
 extern "C" int skm_profile_read(skm_ctx *ctx, const char *h_prefix, int64_t *h_launches, double *h_total_ms)
 {
     SKM_REQUIRE(ctx && h_prefix, SKM_E_BADARG, "null argument");
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     int64_t cnt = 0;
     double tot = 0;
@@ -688,6 +696,7 @@ extern "C" int skm_profile_read(skm_ctx *ctx, const char *h_prefix, int64_t *h_l
 extern "C" int skm_profile_dump(skm_ctx *ctx, char *h_buf, int cap, int *h_needed)
 {
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     std::map<std::string, std::pair<int64_t, double>> agg;
     std::vector<std::string> order;

@@ -696,6 +696,7 @@ extern "C" int skm_basis_build(skm_ctx *ctx, int code_bits, int key_bits, int fl
     SKM_REQUIRE(!p32 || (d_post && d_postcnt && !d_total && n <= ((int64_t)1 << 24)), SKM_E_BADARG,
                 "skm_basis_build: POST32 needs d_post, d_postcnt, no d_total and fewer than 2^24 rows");
     *h_ncols = 0;
+    SKM_ON_DEVICE(ctx);
     if (nnz == 0) {
         if (d_colptr)
             SKM_HIP(hipMemsetAsync(d_colptr, 0, sizeof(uint32_t), ctx->stream));
@@ -704,7 +705,6 @@ extern "C" int skm_basis_build(skm_ctx *ctx, int code_bits, int key_bits, int fl
     SKM_REQUIRE(d_rowptr && d_codes && d_counts && d_colidx, SKM_E_BADARG, "skm_basis_build: null CSR array");
     if (key_bits <= 0 || key_bits > code_bits)
         key_bits = code_bits;
-    SKM_ON_DEVICE(ctx);
 #define SKM_BASIS(K, PW)                                                                                                   \
     return basis_impl<K, PW>(ctx, key_bits, flags, n, nnz, d_rowptr, (const K *)d_codes, d_counts, d_firstpos, h_ncols,  \
                              (K *)d_basis, d_colidx, d_df, d_total, d_firstkey, d_fs_order, d_colptr, (PW *)d_post, d_postcnt)

@@ -146,7 +146,7 @@ extern "C" int skm_comm_init(skm_ctx *ctx, int nranks, int rank, const uint8_t *
 extern "C" int skm_comm_destroy(skm_ctx *ctx)
 {
     if (ctx && ctx->comm && g_rccl.destroy) {
-        hipSetDevice(ctx->device);
+        const skm_device_scope scope(ctx->device, ctx->foreign);
         hipStreamSynchronize(ctx->stream);
         g_rccl.destroy(ctx->comm);
         ctx->comm = nullptr;

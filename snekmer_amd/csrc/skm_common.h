@@ -143,8 +143,10 @@ struct skm_lut256 {
 struct skm_device_scope {
     int before = -1;
     hipError_t err = hipSuccess;
-    skm_device_scope(int device, bool foreign)
+    skm_device_scope(int device, bool foreign)  // device < 0: the current one stays
     {
+        if (device < 0)
+            return;
         if (foreign && (hipGetDevice(&before) != hipSuccess || before == device))
             before = -1;
         err = hipSetDevice(device);
@@ -159,6 +161,10 @@ struct skm_device_scope {
 };
 #define SKM_ON_DEVICE(ctx)                                              \
     const skm_device_scope skm_scope_((ctx)->device, (ctx)->foreign);   \
+    SKM_HIP(skm_scope_.err)
+// For calls that only queue copies or wait: every stream but the null stream, which is the current device's, names its own device.
+#define SKM_ON_STREAM(ctx)                                                                             \
+    const skm_device_scope skm_scope_((ctx)->stream ? -1 : (ctx)->device, (ctx)->foreign);             \
     SKM_HIP(skm_scope_.err)
 
 static inline int64_t skm_ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

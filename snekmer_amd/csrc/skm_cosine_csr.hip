@@ -2100,6 +2100,7 @@ int skm_similarity_to_distance(skm_ctx *ctx, int64_t rows, int64_t m, float *d_o
 {
     if (rows <= 0 || m <= 0)
         return SKM_OK;
+    SKM_ON_DEVICE(ctx);  // (the callers' own scopes have ended)
     dim3 grid((unsigned)skm_ceil_div(m, 256), (unsigned)(rows < 4096 ? rows : 4096));
     SKM_PROF(ctx, "k_similarity_to_distance");
     k_similarity_to_distance<<<grid, 256, 0, ctx->stream>>>(rows, m, d_out, ld);
@@ -2172,6 +2173,7 @@ extern "C" int skm_cosine_csr_phase(skm_ctx *ctx, skm_ctx *exec_ctx, int phase, 
 extern "C" int skm_debug_gram_phases(skm_ctx *ctx, unsigned long long *h_ticks8)
 {
     SKM_REQUIRE(ctx && h_ticks8, SKM_E_BADARG, "skm_debug_gram_phases: bad argument");
+    SKM_ON_STREAM(ctx);
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     SKM_HIP(hipMemcpyFromSymbol(h_ticks8, HIP_SYMBOL(g_gram_phase_ticks), 8 * sizeof(unsigned long long)));
     return SKM_OK;

@@ -1,6 +1,7 @@
 """Parts of the scoring operators that can be checked without a device: index arithmetic of the kernels compiled for the host, and
 what the library's sources and Python layer promise about streams, devices and arguments."""
 import os
+import re
 import shutil
 import subprocess
 
@@ -107,3 +108,37 @@ def test_labels_in_another_librarys_host_memory():
         apply.log_probabilities(Recorder(), S, HostTensor([0, 6, -1, 2]))
     with pytest.raises(TypeError, match="on the device"):  # scores may not
         apply.log_probabilities(Recorder(), HostTensor([[1.0, 2.0]]), [0])
+
+
+# ---------------------------------------------------------------------------- contexts over a caller's stream, as the sources handle them
+def functions_of_the_library():
+    """(file, name, parameters, body) of every function at file scope in the library's sources."""
+    for name in sorted(os.listdir(CSRC)):
+        if not name.endswith(".hip"):
+            continue
+        text = open(os.path.join(CSRC, name)).read()
+        for m in re.finditer(r'^(?:extern "C" |static |template <[^>]*>\s*)*(?:int|bool|void)\s+(\w+)\(([^)]*)\)\s*\{', text, re.M):
+            end = text.index("\n}\n", m.end())
+            yield name, m.group(1), m.group(2), text[m.end():end]
+
+
+def test_every_call_on_a_contexts_stream_is_on_its_device():
+    """The null stream, which a context may be over, is the CURRENT device's, and launches want the stream's device to be the current one:
+    whatever uses a context's stream makes its device current first.  (One device here: the calls' sources are looked at.)"""
+    scopes = ("SKM_ON_DEVICE(", "SKM_ON_STREAM(", "skm_device_scope scope(")
+    # its stream is never the null stream; swaps two contexts' streams of one device and calls what is looked at here
+    exempt = {"skm_graph_end", "skm_cosine_csr_phase"}
+    looked = 0
+    for file, name, parameters, body in functions_of_the_library():
+        if "skm_ctx" not in parameters or name in exempt:
+            continue
+        # entry points, and what they call behind the scope of another function
+        if name.startswith("skm_") and not name.endswith("_async") and name not in ("skm_ws", "skm_pool_alloc", "skm_pool_free", "skm_foreign_capture"):
+            use = re.search(r"(hip[A-Z]\w+\([^;]*|<<<[^;]*|hipStream_t \w+ = )ctx->stream", body)
+            if use is None:
+                continue
+            looked += 1
+            first = min((body.index(s) for s in scopes if s in body), default=None)
+            assert first is not None and first < use.start(), f"{file}: {name}"
+        assert "hipSetDevice" not in body, f"{file}: {name}"  # (the scopes give the caller's device back)
+    assert looked > 60
