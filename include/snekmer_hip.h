@@ -76,8 +76,9 @@ int skm_create(int device_id, skm_ctx **out_ctx);
 int skm_create_confined(int device_id, int first_cu_group, int last_cu_group, skm_ctx **out_ctx);
 /* A context over the caller's own stream (a hipStream_t of `device_id`; NULL: the null stream), e.g. the current stream of
  * another library whose arrays the calls read and write: what both queue there runs in order, with no wait between.  The
- * stream stays the caller's and has to outlive the context.  While its owner captures it, only calls without scratch
- * memory can be made (SKM_E_UNSUPPORTED otherwise): a graph captured with skm_graph_begin knows when it is stale.
+ * stream stays the caller's and has to outlive the context.  While its owner captures it, only calls can be made that need
+ * no scratch memory and neither wait, fill, replay a graph nor free the context (SKM_E_UNSUPPORTED otherwise): a graph captured
+ * with skm_graph_begin knows when it is stale.
  * skm_pointer_device: the device whose memory d_ptr points into, -1 for anything else.  No reference counterparts. */
 int skm_create_on_stream(int device_id, void *stream, skm_ctx **out_ctx);
 int skm_pointer_device(const void *d_ptr, int *h_device);

@@ -20,6 +20,7 @@ LIB_PATH = os.environ.get("SNEKMER_HIP_LIB") or os.path.join(_HERE, "libsnekmer_
 SKM_OK = 0
 ABI_VERSION = 8  # SKM_ABI_VERSION of include/snekmer_hip.h
 ERRORS = {-1: "BADARG", -2: "NOMEM", -3: "HIP", -4: "OVERFLOW", -5: "UNSUPPORTED", -6: "COMM", -7: "STALE"}
+UNSUPPORTED = -5
 COMM_ID_BYTES = 128
 EVENT_SLOTS = 8  # SKM_EVENT_SLOTS
 
@@ -480,12 +481,19 @@ class Context:
     def close(self):
         """Free the context.  Pinned host memory handed out by host_alloc (the small-batch arena of engine.py
         included) is freed with it: numpy views a caller kept over it are dangling afterwards, and any later call on
-        this context raises."""
+        this context raises.  While the owner of the context's stream captures it, nothing is freed and the call raises: work that
+        was queued before may still use what the context holds."""
         if getattr(self, "handle", None) is not None:
-            self.__dict__.pop("_arena", None)  # its views point into the pinned memory freed below
-            for ptr in self.__dict__.pop("_pinned", []):
-                self.lib.skm_host_free(self.handle, _p(ptr))
-            self.lib.skm_destroy(self.handle)
+            pinned = self.__dict__.get("_pinned", [])
+            while pinned:
+                status = self.lib.skm_host_free(self.handle, _p(pinned[-1]))
+                if status == UNSUPPORTED:
+                    _check(self.lib, status)
+                self.__dict__.pop("_arena", None)  # its views point into the pinned memory that goes
+                pinned.pop()
+            status = self.lib.skm_destroy(self.handle)
+            if status == UNSUPPORTED:
+                _check(self.lib, status)
             self.handle = None
 
     def __del__(self):

@@ -247,6 +247,7 @@ extern "C" int skm_destroy(skm_ctx *ctx)
     if (!ctx)
         return SKM_OK;
     const skm_device_scope scope(ctx->device, ctx->foreign);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_destroy");
     if (ctx->capturing) {  // an abandoned capture: end it so that the stream can be waited for and reused
         hipGraph_t g = nullptr;
         if (hipStreamEndCapture(ctx->stream, &g) == hipSuccess && g)
@@ -358,6 +359,7 @@ extern "C" int skm_sync(skm_ctx *ctx)
 {
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     SKM_ON_STREAM(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_sync");
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     return skm_check_device_error(ctx, "skm_sync");
 }
@@ -426,6 +428,7 @@ extern "C" int skm_host_free(skm_ctx *ctx, void *hptr)
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     if (hptr) {
         SKM_ON_DEVICE(ctx);
+        SKM_NOT_WHILE_CAPTURED(ctx, "skm_host_free");
         SKM_TRY(skm_quiesce_device(ctx->device));  // kernels read and write this memory in place; the wait is explicit
         SKM_HIP(hipHostFree(hptr));
     }
@@ -438,6 +441,7 @@ extern "C" int skm_memcpy_h2d(skm_ctx *ctx, void *d_dst, const void *h_src, size
     if (!bytes)
         return SKM_OK;
     SKM_ON_STREAM(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_memcpy_h2d");
     SKM_HIP(hipMemcpyAsync(d_dst, h_src, bytes, hipMemcpyHostToDevice, ctx->stream));
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     return SKM_OK;
@@ -460,6 +464,7 @@ extern "C" int skm_memcpy_d2h(skm_ctx *ctx, void *h_dst, const void *d_src, size
     if (!bytes)
         return SKM_OK;
     SKM_ON_STREAM(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_memcpy_d2h");
     SKM_HIP(hipMemcpyAsync(h_dst, d_src, bytes, hipMemcpyDeviceToHost, ctx->stream));
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     return skm_check_device_error(ctx, "skm_memcpy_d2h");
@@ -481,6 +486,7 @@ extern "C" int skm_memset(skm_ctx *ctx, void *d_dst, int byte_value, size_t byte
     if (!bytes)
         return SKM_OK;
     SKM_ON_STREAM(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_memset");
     SKM_HIP(hipMemsetAsync(d_dst, byte_value, bytes, ctx->stream));
     return SKM_OK;
 }
@@ -604,6 +610,7 @@ extern "C" int skm_graph_launch(skm_ctx *ctx, skm_graph *graph)
         return SKM_E_STALE;
     }
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_graph_launch");
     SKM_HIP(hipGraphLaunch(graph->exec, ctx->stream));
     return SKM_OK;
 }
@@ -616,6 +623,7 @@ extern "C" int skm_graph_destroy(skm_ctx *ctx, skm_graph *graph)
     auto it = std::find(ctx->graphs.begin(), ctx->graphs.end(), graph);
     SKM_REQUIRE(it != ctx->graphs.end(), SKM_E_BADARG, "skm_graph_destroy: not a live graph of this context");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_graph_destroy");  // (skm_destroy will release it)
     (void)hipStreamSynchronize(ctx->stream);  // a replay may still be running
     ctx->graphs.erase(it);
     skm_graph_release(graph);
@@ -625,7 +633,7 @@ extern "C" int skm_graph_destroy(skm_ctx *ctx, skm_graph *graph)
 // ---------------------------------------------------------------------------- profiling
 skm_prof_scope::skm_prof_scope(skm_ctx *c, const char *name, hipStream_t on) : ctx(c), st(on ? on : c->stream)
 {
-    if (!ctx->profiling || ctx->capturing)
+    if (!ctx->profiling || ctx->capturing || skm_foreign_capture(ctx))
         return;
     skm_prof_entry ent;
     ent.name = name;
@@ -661,6 +669,7 @@ extern "C" int skm_profile_reset(skm_ctx *ctx)
 {
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     SKM_ON_STREAM(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_profile_reset");
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     for (auto &p : ctx->prof) {
         ctx->event_pool.push_back(p.start);
@@ -674,6 +683,7 @@ extern "C" int skm_profile_read(skm_ctx *ctx, const char *h_prefix, int64_t *h_l
 {
     SKM_REQUIRE(ctx && h_prefix, SKM_E_BADARG, "null argument");
     SKM_ON_STREAM(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_profile_read");
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     int64_t cnt = 0;
     double tot = 0;
@@ -697,6 +707,7 @@ extern "C" int skm_profile_dump(skm_ctx *ctx, char *h_buf, int cap, int *h_neede
 {
     SKM_REQUIRE(ctx, SKM_E_BADARG, "null context");
     SKM_ON_STREAM(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_profile_dump");
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     std::map<std::string, std::pair<int64_t, double>> agg;
     std::vector<std::string> order;

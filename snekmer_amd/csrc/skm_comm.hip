@@ -147,6 +147,7 @@ extern "C" int skm_comm_destroy(skm_ctx *ctx)
 {
     if (ctx && ctx->comm && g_rccl.destroy) {
         const skm_device_scope scope(ctx->device, ctx->foreign);
+        SKM_NOT_WHILE_CAPTURED(ctx, "skm_comm_destroy");
         hipStreamSynchronize(ctx->stream);
         g_rccl.destroy(ctx->comm);
         ctx->comm = nullptr;

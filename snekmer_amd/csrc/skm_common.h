@@ -98,6 +98,9 @@ hipError_t skm_pinned_acquire(int device, void **out_page4096);
 void skm_pinned_release(int device, void *page);
 // true while the owner of a foreign stream captures it (not through skm_graph_begin): nothing there may be queried or waited for
 bool skm_foreign_capture(const skm_ctx *ctx);
+// Calls that wait for the stream, replay a graph on it or let go of what its work uses: made inside the owner's capture they would end it.
+#define SKM_NOT_WHILE_CAPTURED(ctx, who) \
+    SKM_REQUIRE(!skm_foreign_capture(ctx), SKM_E_UNSUPPORTED, "%s: the owner of the context's stream captures it", who)
 void skm_graph_release(struct skm_graph *graph);
 constexpr int SKM_DEVERR_WORD = 768;  // byte 3072 of h_pinned
 enum skm_deverr { SKM_DEVERR_SEQ_TOO_LONG = 0, SKM_DEVERR_LABEL, SKM_DEVERR_COUNT };

@@ -2039,6 +2039,7 @@ extern "C" int skm_cosine_csr_stats(skm_ctx *ctx, int64_t *h_out4)
     if (!ctx->ws[WS_COS] || ctx->ws_bytes[WS_COS] < sizeof(cos_state))
         return SKM_OK;
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_cosine_csr_stats");
     cos_state host;
     SKM_HIP(hipMemcpyAsync(&host, ctx->ws[WS_COS], offsetof(cos_state, pad), hipMemcpyDeviceToHost, ctx->stream));
     SKM_HIP(hipStreamSynchronize(ctx->stream));
@@ -2061,6 +2062,7 @@ extern "C" int skm_heavy_panel_stats(skm_ctx *ctx, int64_t *h_out6)
     if (!ctx->panel_meta || ctx->panel_nb <= 0)
         return SKM_OK;
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_heavy_panel_stats");
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     std::vector<uint32_t> meta(4 * (size_t)ctx->panel_nb);
     uint32_t rows = 0;
@@ -2146,6 +2148,8 @@ extern "C" int skm_cosine_csr_phase(skm_ctx *ctx, skm_ctx *exec_ctx, int phase, 
     SKM_REQUIRE(post_bits == 64 || post_bits == 32, SKM_E_BADARG, "skm_cosine_csr_phase: post_bits must be 32 or 64");
     SKM_REQUIRE(mode >= 0 && mode <= 2, SKM_E_BADARG, "skm_cosine_csr_phase: mode must be 0, 1 or 2");
     SKM_REQUIRE(!exec_ctx || exec_ctx->device == ctx->device, SKM_E_BADARG, "skm_cosine_csr_phase: the two contexts are on different devices");
+    if (exec_ctx)  // (ctx's scratch in a graph of the other stream's owner)
+        SKM_NOT_WHILE_CAPTURED(exec_ctx, "skm_cosine_csr_phase");
     if (post_bits == 32)
         SKM_REQUIRE(m <= ((int64_t)1 << 24), SKM_E_BADARG, "skm_cosine_csr_phase: 32-bit postings hold rows < 2^24");
     struct stream_swap {  // phase 2: ctx's kernels, scratch and profiling scopes, on exec_ctx's stream
@@ -2174,6 +2178,7 @@ extern "C" int skm_debug_gram_phases(skm_ctx *ctx, unsigned long long *h_ticks8)
 {
     SKM_REQUIRE(ctx && h_ticks8, SKM_E_BADARG, "skm_debug_gram_phases: bad argument");
     SKM_ON_STREAM(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_debug_gram_phases");
     SKM_HIP(hipStreamSynchronize(ctx->stream));
     SKM_HIP(hipMemcpyFromSymbol(h_ticks8, HIP_SYMBOL(g_gram_phase_ticks), 8 * sizeof(unsigned long long)));
     return SKM_OK;

@@ -957,6 +957,7 @@ extern "C" int skm_recode(skm_ctx *ctx, const uint8_t *h_translate, const uint8_
     if (n == 0)
         return SKM_OK;
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_recode");
     int64_t *h_tot = (int64_t *)ctx->h_pinned;
     SKM_HIP(hipMemcpyAsync(h_tot, d_off + n, sizeof(int64_t), hipMemcpyDeviceToHost, ctx->stream));
     SKM_HIP(hipStreamSynchronize(ctx->stream));

@@ -485,7 +485,7 @@ int skm_pool_free(skm_ctx *ctx, void *ptr)
         lb = it->second;
     }
     int rc = SKM_OK;
-    if (lb.guarded && !ctx->capturing) {
+    if (lb.guarded && !ctx->capturing && !skm_foreign_capture(ctx)) {
         // (outside the lock: a host wait)  every stream that may have written the array must be done before the look
         unsigned char host[GUARD_BYTES];
         SKM_TRY(skm_quiesce_device(ctx->device));

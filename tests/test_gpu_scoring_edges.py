@@ -287,7 +287,9 @@ def test_arrays_without_cells_need_no_address(ctx):
 
 
 # ---------------------------------------------------------------------------- beside other libraries
-def test_while_torch_captures():
-    """tests/torch_interop_edges.py, in a process that loads torch first."""
-    run = subprocess.run([sys.executable, "-u", os.path.join(os.path.dirname(__file__), "torch_interop_edges.py")], capture_output=True, text=True, timeout=110)
+@pytest.mark.parametrize("guard", ["0", "1"])
+def test_while_torch_captures(guard):
+    """tests/torch_interop_edges.py, in a process that loads torch first; with and without the bytes that guard the ends of arrays."""
+    run = subprocess.run([sys.executable, "-u", os.path.join(os.path.dirname(__file__), "torch_interop_edges.py")], capture_output=True, text=True, timeout=110,
+                         env=dict(os.environ, SKM_GUARD=guard))
     assert run.returncode == 0 and run.stdout.rstrip().endswith("all passed"), run.stdout + run.stderr

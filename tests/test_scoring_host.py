@@ -142,3 +142,20 @@ def test_every_call_on_a_contexts_stream_is_on_its_device():
             assert first is not None and first < use.start(), f"{file}: {name}"
         assert "hipSetDevice" not in body, f"{file}: {name}"  # (the scopes give the caller's device back)
     assert looked > 60
+
+
+def test_nothing_waits_for_a_stream_that_its_owner_captures():
+    """A wait inside the owner's capture ends the capture: every function that waits has asked first, by itself or by asking for scratch
+    memory, which is refused then."""
+    asks = ("SKM_NOT_WHILE_CAPTURED(", "skm_ws(", "skm_foreign_capture(")
+    # waits of the pool (for streams that it has asked about) and at the end of the process
+    exempt = {"park_locked", "quiesce_locked", "skm_stream_release", "shutdown_at_exit"}
+    looked = 0
+    for file, name, parameters, body in functions_of_the_library():
+        wait = re.search(r"hip(Stream|Event)Synchronize\(", body)
+        if wait is None or name in exempt:
+            continue
+        looked += 1
+        first = min((body.index(a) for a in asks if a in body), default=None)
+        assert first is not None and first < wait.start(), f"{file}: {name}"
+    assert looked > 20

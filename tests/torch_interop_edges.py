@@ -68,7 +68,48 @@ def a_graph_that_outlives_its_context():
         other.close()
 
 
-for check in (a_graph_that_outlives_its_context,):
+def calls_that_would_end_a_capture():
+    """Inside torch's capture: waits, copies that wait, fills, replays and the context's end are refused, timing records nothing, arrays may
+    go; the capture ends well and its replays are right, and so is the context."""
+    s = torch.cuda.Stream()
+    own = _hip.Context(0, stream=s.cuda_stream)
+    with torch.cuda.stream(s):
+        x = torch.ones(500, 64, dtype=torch.bfloat16, device="cuda")
+        w = torch.ones(300, 64, dtype=torch.bfloat16, device="cuda")
+        y, z = (torch.empty(500, 300, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        engine.linear(own, x, w, out=z)  # (whatever the call needs at first)
+        own.graph_begin()
+        engine.linear(own, x, w, out=z)
+        recorded = own.graph_end()
+        kept, going = own.to_device(np.arange(100, dtype=np.float32)), own.to_device(np.arange(100, dtype=np.float32))
+        pinned = own.host_alloc(64)
+        own.profile_enable(True)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            engine.linear(own, x, w, out=y)
+            for call in (own.sync, kept.download, lambda: kept.upload(np.zeros(100, np.float32)), lambda: own.profile_read("k_linear"), own.profile_reset, own.profile_dump,
+                         recorded.launch, own.close, lambda: own.call("skm_memset", kept.ptr, 0, 400)):
+                raises(_hip.HipError, "captures", call)
+            assert own.lib.skm_graph_destroy(own.handle, recorded.handle) == _hip.UNSUPPORTED
+            del going
+        own.profile_enable(False)
+        for value in (2.0, 1.0, 3.0):
+            x.fill_(value)
+            y.zero_()
+            z.zero_()
+            g.replay()
+            recorded.launch()
+            own.sync()
+            assert bool((y == 64 * value).all()) and bool((z == 64 * value).all())
+        assert own.profile_read("k_linear")[0] == 0
+        assert np.array_equal(kept.download(), np.arange(100, dtype=np.float32))
+        pinned[:] = 7
+        recorded.close()
+    own.close()
+
+
+for check in (a_graph_that_outlives_its_context, calls_that_would_end_a_capture):
     print(check.__name__, flush=True)
     check()
 print("all passed", flush=True)
