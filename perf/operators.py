@@ -12,7 +12,7 @@ own = False
 DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 SIZES = {"f32": 4, "f16": 2, "bf16": 2}
 ACTIVATIONS = ("none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid")
-_context = None
+_contexts = {}
 
 
 def _logp(name, rows, cols, dtype, k, kind, mask="none", temperature=1.0, pad=0):
@@ -283,27 +283,28 @@ def _plain_linear_grad(state, kind=torch.float32):
 
 # ---------------------------------------------------------------------------- one pass
 def _own_run(state):
-    """The framework's calls, on a context over torch's own stream, into the caller's arrays."""
-    global _context
+    """The framework's calls, on a context over torch's current stream, into the caller's arrays."""
     from snekmer_amd import _hip, apply, engine
 
-    if _context is None:
-        _context = _hip.Context(torch.cuda.current_device(), stream=torch.cuda.current_stream().cuda_stream)
+    where = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+    context = _contexts.get(where)
+    if context is None:
+        context = _contexts[where] = _hip.Context(where[0], stream=where[1])
     case = state["case"]
     if case["op"] == "logp":
         out = apply.LogProbabilities(**state["out"])
-        apply.log_probabilities(_context, state["scores"], state["labels"], k=case["k"], temperature=case["temperature"], mask=state["mask"], out=out)
+        apply.log_probabilities(context, state["scores"], state["labels"], k=case["k"], temperature=case["temperature"], mask=state["mask"], out=out)
         return state["out"]
     if case["op"] == "logp_grad":
         forward = apply.LogProbabilities(stats=state["stats"], entropy=state["entropy"])
-        apply.log_probabilities_backward(_context, state["scores"], state["labels"], forward, d_logp=state["d_logp"], d_entropy=state["d_entropy"],
+        apply.log_probabilities_backward(context, state["scores"], state["labels"], forward, d_logp=state["d_logp"], d_entropy=state["d_entropy"],
                                          temperature=case["temperature"], mask=state["mask"], out=state["out"])
         return state["out"]
     if case["op"] == "linear":
-        engine.linear(_context, state["x"], state["w"], bias=state["bias"], activation=case["activation"], residual=state["residual"],
+        engine.linear(context, state["x"], state["w"], bias=state["bias"], activation=case["activation"], residual=state["residual"],
                       preact=state["preact"], out=state["out"])
         return {"y": state["out"], "preact": state["preact"]} if case["preact"] else {"y": state["out"]}
-    engine.linear_backward(_context, state["dy"], state["x"], state["w"], activation=case["activation"], preact=state["preact"],
+    engine.linear_backward(context, state["dy"], state["x"], state["w"], activation=case["activation"], preact=state["preact"],
                            dx=state["dx"], dw=state["dw"], dbias=state["dbias"])
     return {"dx": state["dx"], "dw": state["dw"], "dbias": state["dbias"]}
 
