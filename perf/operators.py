@@ -286,7 +286,8 @@ def _own_run(state):
     """The framework's calls, on a context over torch's current stream, into the caller's arrays."""
     from snekmer_amd import _hip, apply, engine
 
-    where = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+    device = torch.cuda.current_device()
+    where = device, torch._C._cuda_getCurrentRawStream(device)  # (torch.cuda.current_stream().cuda_stream: 2.8 us instead of 0.1)
     context = _contexts.get(where)
     if context is None:
         context = _contexts[where] = _hip.Context(where[0], stream=where[1])
