@@ -379,6 +379,10 @@ def is_device_array(x) -> bool:
 _TENSOR_TYPES = {}  # type string by dtype object, of arrays that also answer data_ptr() / stride() (see array_view)
 
 
+def _no() -> bool:
+    return False
+
+
 def array_view(ctx: "Context", x, name: str, ndim: int, types, writable: bool = False):
     """(pointer, shape, row stride in elements, type string) of a device array of this library or of another one
     (`__cuda_array_interface__`), as the entry points take them: the elements of a row next to each other, rows that do not
@@ -408,6 +412,9 @@ def array_view(ctx: "Context", x, name: str, ndim: int, types, writable: bool = 
     if len(shape) != ndim:
         raise ValueError(f"{name}: {len(shape)} dimensions, want {ndim}")
     cols = shape[-1]
+    # (views whose values are the negated words: the imaginary parts of conjugated numbers, whose strides only single columns hide)
+    if cols == 1 and getattr(x, "is_neg", _no)():
+        raise ValueError(f"{name}: a view of negated values; resolve it first")
     ld = cols
     if strides is not None:
         if cols > 1 and strides[-1] != 1:

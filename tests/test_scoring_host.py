@@ -110,6 +110,20 @@ def test_labels_in_another_librarys_host_memory():
         apply.log_probabilities(Recorder(), HostTensor([[1.0, 2.0]]), [0])
 
 
+def test_views_of_negated_values_are_refused():
+    """torch's imag of conj: the words in memory have the other sign.  Elements two apart are refused as such; one column has none."""
+
+    class Negated(Fake):
+        def is_neg(self):
+            return True
+
+    for view, ndim in ((Negated((3, 1), strides=(8, 8)), 2), (Negated((1,)), 1)):
+        with pytest.raises(ValueError, match="x: a view of negated"):
+            _hip.array_view(CTX, view, "x", ndim, _hip.FLOAT_TYPES)
+    Negated.is_neg = lambda self: False
+    assert _hip.array_view(CTX, Negated((3, 1), strides=(8, 8)), "x", 2, _hip.FLOAT_TYPES)[2] == 2
+
+
 # ---------------------------------------------------------------------------- contexts over a caller's stream, as the sources handle them
 def functions_of_the_library():
     """(file, name, parameters, body) of every function at file scope in the library's sources."""
