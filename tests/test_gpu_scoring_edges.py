@@ -293,3 +293,52 @@ def test_while_torch_captures(guard):
     run = subprocess.run([sys.executable, "-u", os.path.join(os.path.dirname(__file__), "torch_interop_edges.py")], capture_output=True, text=True, timeout=110,
                          env=dict(os.environ, SKM_GUARD=guard))
     assert run.returncode == 0 and run.stdout.rstrip().endswith("all passed"), run.stdout + run.stderr
+
+
+# ---------------------------------------------------------------------------- as they are used together
+@pytest.mark.parametrize("alpha, k, full", [("solvacc", 6, True), ("red6", 5, False), ("hydro", 7, True)])
+def test_a_head_over_the_counts_of_sequences(ctx, alpha, k, full):
+    """Sequences -> k-mer counts -> dense rows (the whole basis, or the one that was observed) -> scores of a head -> log probabilities of the
+    families -> gradients, all on the device; each step against float64 from what the step before it left, the gradient against the formula."""
+    from helpers import ensure_red6
+    from snekmer_amd import alphabet
+    from snekmer_amd.synth import synth_families
+
+    ensure_red6()
+    lut = alphabet.build_lut(alpha)
+    n, a = 300, 15
+    res, off, _ = synth_families(n, 90, family=20, seed=4)
+    batch = engine.SeqBatch(ctx, res, off)
+    csr = engine.count_csr(ctx, batch, lut, k)
+    if full:
+        width = lut.nsym ** k
+        x = engine.csr_to_dense(ctx, n, csr.rowptr, csr.codes, csr.counts, width, dtype=np.float32)
+    else:
+        basis = engine.build_basis(ctx, csr, lut.nsym, k)
+        width = basis.ncols
+        x = engine.csr_to_dense(ctx, n, csr.rowptr, csr.colidx, csr.counts, width, dtype=np.float32)
+    rowptr, counts = csr.rowptr.download(n + 1), csr.counts.download(csr.nnz)
+    columns = (csr.codes if full else csr.colidx).download(csr.nnz).astype(np.int64)
+    dense = np.zeros((n, width))
+    dense[np.repeat(np.arange(n), np.diff(rowptr)), columns] = counts
+    assert np.array_equal(x.download(), dense) and dense.sum() > 50 * n
+    rng = np.random.default_rng(k)
+    w, b = (rng.normal(size=(a, width)) / 8).astype(np.float32), rng.normal(size=a).astype(np.float32)
+    groups = np.arange(n) // 20
+    dw_, db_ = ctx.to_device(w), ctx.to_device(b)
+    z = engine.linear(ctx, x, dw_, bias=db_)
+    w64, z32 = w.astype(np.float64), z.download().astype(np.float64)
+    room = (width + 2) * U * (dense @ np.abs(w64).T + np.abs(b))
+    assert (np.abs(z32 - (dense @ w64.T + b)) <= room).all()
+    T = 0.8
+    lp = apply.log_probabilities(ctx, z, groups, k=3, temperature=T)
+    want = plain_logp(z32, groups, 3, T)
+    check_logp(lp.host(), want, a, T, 3)
+    ds = apply.log_probabilities_backward(ctx, z, groups, lp, d_logp=ctx.to_device(np.full(n, -1.0 / n, np.float32)), temperature=T)
+    g = ds.download().astype(np.float64)
+    exact = exact_gradient(want, groups, np.full(n, -1.0 / n), np.zeros(n), T)
+    # p: (4 |d| + 4 l + 8) u and what l is off, (16 + 90 + 4 l) u: all |d| below 2^7 here
+    assert (np.abs(g - exact) <= 2.0 ** -13 * (want["p"] + (np.arange(a) == groups[:, None])) / (n * T)).all()
+    dx, dw, db = (v.download().astype(np.float64) for v in engine.linear_backward(ctx, ds, x, dw_))
+    for got, left, right, length in ((dx, g, w64, a), (dw, g.T, dense, n), (db[None], np.ones((1, n)), g, n)):
+        assert (np.abs(got - left @ right) <= (length + 2) * U * (np.abs(left) @ np.abs(right)) + 2.0 ** -140).all()
