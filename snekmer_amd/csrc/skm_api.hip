@@ -758,6 +758,7 @@ extern "C" int skm_vectorize_csr(skm_ctx *ctx, const uint8_t *h_rank, int nsym, 
     SKM_REQUIRE(total_residues < ((int64_t)1 << 32) - 1 && n < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW,
                 "skm_vectorize_csr: more than 2^32 residues or sequences in one batch; split the batch");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_vectorize_csr");
     if (counts_only)
         return skm_count_stage_async(ctx, h_rank, nsym, k, code_bits, d_seq, d_off, n, total_residues, max_seq_len, d_rowptr, d_codes, d_counts,
                                      nullptr, d_rnorm, d_normsq);

@@ -697,6 +697,7 @@ extern "C" int skm_basis_build(skm_ctx *ctx, int code_bits, int key_bits, int fl
                 "skm_basis_build: POST32 needs d_post, d_postcnt, no d_total and fewer than 2^24 rows");
     *h_ncols = 0;
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_basis_build");
     if (nnz == 0) {
         if (d_colptr)
             SKM_HIP(hipMemsetAsync(d_colptr, 0, sizeof(uint32_t), ctx->stream));
@@ -727,6 +728,7 @@ extern "C" int skm_csr_transpose(skm_ctx *ctx, int64_t n, int64_t nnz, int64_t n
     SKM_REQUIRE(nnz < ((int64_t)1 << 32) - 1 && ncols < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW,
                 "skm_csr_transpose: nnz or ncols >= 2^32");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_csr_transpose");
     hipStream_t st = ctx->stream;
     if (nnz == 0) {
         SKM_HIP(hipMemsetAsync(d_colptr, 0, sizeof(uint32_t) * (size_t)(ncols + 1), st));
@@ -788,6 +790,7 @@ extern "C" int skm_csr_to_dense(skm_ctx *ctx, int64_t n, const int64_t *d_rowptr
         return SKM_OK;
     SKM_REQUIRE(d_rowptr && d_out, SKM_E_BADARG, "skm_csr_to_dense: null array");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_csr_to_dense");
     const size_t esz = dtype == 0 ? 8 : (dtype == 1 ? 4 : 1);
     SKM_HIP(hipMemsetAsync(d_out, 0, esz * (size_t)n * (size_t)ld, ctx->stream));
     const int grid = skm_grid_cap(ctx, skm_ceil_div(n, BLK / 64), 16);
@@ -957,6 +960,7 @@ extern "C" int skm_csr_max_count_dev(skm_ctx *ctx, int64_t n, int64_t cap_entrie
 {
     SKM_REQUIRE(ctx && n >= 0 && cap_entries >= 0 && d_rowptr && d_out_max, SKM_E_BADARG, "skm_csr_max_count_dev: bad argument");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_csr_max_count_dev");
     SKM_HIP(hipMemsetAsync(d_out_max, 0, 4, ctx->stream));
     if (cap_entries == 0)
         return SKM_OK;

@@ -1279,6 +1279,7 @@ extern "C" int skm_dense_to_csr(skm_ctx *ctx, int64_t n, int64_t ncols, int dtyp
     SKM_REQUIRE(dtype >= 0 && dtype <= 2, SKM_E_BADARG, "skm_dense_to_csr: dtype must be 0 (uint16), 1 (uint32) or 2 (int8)");
     SKM_REQUIRE(ncols < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW, "skm_dense_to_csr: ncols >= 2^32");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_dense_to_csr");
     hipStream_t st = ctx->stream;
     *h_nnz = 0;
     if (n == 0 || ncols == 0) {
@@ -1466,6 +1467,7 @@ extern "C" int skm_csr_to_dense_i8(skm_ctx *ctx, int64_t n, const int64_t *d_row
     SKM_REQUIRE(ctx && n >= 0 && kdim >= 0 && kdim % 64 == 0, SKM_E_BADARG, "skm_csr_to_dense_i8: bad argument (kdim must be a multiple of 64)");
     SKM_REQUIRE(d_irr_count, SKM_E_BADARG, "skm_csr_to_dense_i8: null counter");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_csr_to_dense_i8");
     SKM_HIP(hipMemsetAsync(d_irr_count, 0, sizeof(uint32_t), ctx->stream));
     if (n == 0 || kdim == 0)
         return SKM_OK;

@@ -193,6 +193,7 @@ extern "C" int skm_csr_remap_columns(skm_ctx *ctx, int64_t n, const int64_t *d_r
 {
     SKM_REQUIRE(ctx && n >= 0 && ncols >= 0 && d_out_rowptr && h_out_nnz, SKM_E_BADARG, "skm_csr_remap_columns: bad argument");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_csr_remap_columns");
     hipStream_t st = ctx->stream;
     *h_out_nnz = 0;
     if (n == 0) {

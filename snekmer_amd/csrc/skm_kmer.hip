@@ -1024,6 +1024,7 @@ extern "C" int skm_count_csr(skm_ctx *ctx, const uint8_t *h_rank, int nsym, int 
     SKM_TRY(make_lut(h_rank, &lut));
     SKM_TRY(check_code_space(nsym, k, code_bits));
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_count_csr");
     *h_nnz = 0;
     if (n == 0) {
         SKM_HIP(hipMemsetAsync(d_rowptr, 0, sizeof(int64_t), ctx->stream));

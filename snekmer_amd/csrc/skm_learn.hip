@@ -379,6 +379,7 @@ extern "C" int skm_group_postings(skm_ctx *ctx, int64_t n, int64_t ncols, const 
     SKM_REQUIRE(nnz < ((int64_t)1 << 32) - 1 && ncols < ((int64_t)1 << 32) - 1 && ngroups < ((int64_t)1 << 32) - 2, SKM_E_OVERFLOW,
                 "skm_group_postings: too large");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_group_postings");
     hipStream_t st = ctx->stream;
     *h_out_nnz = 0;
     if (d_out_normsq && ngroups)
@@ -437,6 +438,7 @@ extern "C" int skm_postings_to_csr(skm_ctx *ctx, int64_t ncols, int64_t nnz, con
     SKM_REQUIRE(ctx && ncols >= 0 && nnz >= 0 && nrows >= 0 && d_out_rowptr, SKM_E_BADARG, "skm_postings_to_csr: bad argument");
     SKM_REQUIRE(nnz < ((int64_t)1 << 32) - 1 && nrows < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW, "skm_postings_to_csr: too large");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_postings_to_csr");
     hipStream_t st = ctx->stream;
     if (nnz == 0) {
         SKM_HIP(hipMemsetAsync(d_out_rowptr, 0, sizeof(int64_t) * (size_t)(nrows + 1), st));
@@ -497,6 +499,7 @@ extern "C" int skm_csr_group_sum(skm_ctx *ctx, int64_t n, int64_t nnz, const int
                 "skm_csr_group_sum: bad argument");
     SKM_REQUIRE(nnz < ((int64_t)1 << 32) - 1 && ngroups < ((int64_t)1 << 32) - 2, SKM_E_OVERFLOW, "skm_csr_group_sum: too large");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_csr_group_sum");
     hipStream_t st = ctx->stream;
     *h_out_nnz = 0;
     if (nnz == 0) {

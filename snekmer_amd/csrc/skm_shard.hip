@@ -354,6 +354,7 @@ extern "C" int skm_bucket_partition(skm_ctx *ctx, int code_bits, int nbuckets, i
     SKM_REQUIRE(cap_entries < ((int64_t)1 << 30) && row_base + n < ((int64_t)1 << 32) - 1, SKM_E_OVERFLOW,
                 "skm_bucket_partition: 2^30 entries or more in one shard, or a row index >= 2^32");
     SKM_ON_DEVICE(ctx);
+    SKM_NOT_WHILE_CAPTURED(ctx, "skm_bucket_partition");
     if (h_counts)
         for (int b = 0; b < nbuckets; ++b)
             h_counts[b] = 0;

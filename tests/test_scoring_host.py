@@ -158,10 +158,13 @@ def test_every_call_on_a_contexts_stream_is_on_its_device():
     assert looked > 60
 
 
+ASKS = ("SKM_NOT_WHILE_CAPTURED(", "skm_ws(", "skm_foreign_capture(")
+
+
 def test_nothing_waits_for_a_stream_that_its_owner_captures():
     """A wait inside the owner's capture ends the capture: every function that waits has asked first, by itself or by asking for scratch
     memory, which is refused then."""
-    asks = ("SKM_NOT_WHILE_CAPTURED(", "skm_ws(", "skm_foreign_capture(")
+    asks = ASKS
     # waits of the pool (for streams that it has asked about) and at the end of the process
     exempt = {"park_locked", "quiesce_locked", "skm_stream_release", "shutdown_at_exit"}
     looked = 0
@@ -173,3 +176,17 @@ def test_nothing_waits_for_a_stream_that_its_owner_captures():
         first = min((body.index(a) for a in asks if a in body), default=None)
         assert first is not None and first < wait.start(), f"{file}: {name}"
     assert looked > 20
+
+
+def test_no_fill_is_recorded_into_an_owners_capture():
+    """Fills that a stream capture records have given wrong results on replays after the first: whoever fills has asked, too."""
+    exempt = {"skm_count_stage_async"}  # (behind skm_count_csr and skm_vectorize_csr)
+    looked = 0
+    for file, name, parameters, body in functions_of_the_library():
+        fill = re.search(r"hipMemsetAsync\(", body)
+        if fill is None or name in exempt:
+            continue
+        looked += 1
+        first = min((body.index(a) for a in ASKS if a in body), default=None)
+        assert first is not None and first < fill.start(), f"{file}: {name}"
+    assert looked > 15

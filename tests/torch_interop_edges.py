@@ -83,13 +83,15 @@ def calls_that_would_end_a_capture():
         recorded = own.graph_end()
         kept, going = own.to_device(np.arange(100, dtype=np.float32)), own.to_device(np.arange(100, dtype=np.float32))
         pinned = own.host_alloc(64)
+        csr = [own.to_device(np.array(v, t)) for v, t in (([0, 1, 3], np.int64), ([2, 0, 3], np.uint32), ([1, 5, 2], np.uint32))]
+        dense = engine.csr_to_dense(own, 2, *csr, 4, dtype=np.float32)
         own.profile_enable(True)
         s.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=s):
             engine.linear(own, x, w, out=y)
             for call in (own.sync, kept.download, lambda: kept.upload(np.zeros(100, np.float32)), lambda: own.profile_read("k_linear"), own.profile_reset, own.profile_dump,
-                         recorded.launch, own.close, lambda: own.call("skm_memset", kept.ptr, 0, 400)):
+                         recorded.launch, own.close, lambda: engine.csr_to_dense(own, 2, *csr, 4, dtype=np.float32, out=dense), lambda: own.call("skm_memset", kept.ptr, 0, 400)):
                 raises(_hip.HipError, "captures", call)
             assert own.lib.skm_graph_destroy(own.handle, recorded.handle) == _hip.UNSUPPORTED
             del going
@@ -104,6 +106,7 @@ def calls_that_would_end_a_capture():
             assert bool((y == 64 * value).all()) and bool((z == 64 * value).all())
         assert own.profile_read("k_linear")[0] == 0
         assert np.array_equal(kept.download(), np.arange(100, dtype=np.float32))
+        assert np.array_equal(dense.download(), [[0, 0, 1, 0], [5, 0, 0, 2]])
         pinned[:] = 7
         recorded.close()
     own.close()
