@@ -431,7 +431,7 @@ int skm_linear(skm_ctx *ctx, int dtype, int activation, int64_t m, int64_t n, in
 
 /* dz = dy act'(preact): dx = dz w, dw = dz^T x, dbias = column sums of dz, each in the operands' type; NULL: not wanted
  * (then w, or x, may be NULL too).  The residual's gradient is dy.  dz is rounded to that type once for the two products
- * (dbias sums the unrounded values).  d_preact is only read where activation is not 0.  No output may share memory with an
+ * (in 16 bits dx and dw are off by 1.4 times what their own rounding costs; dbias sums the unrounded values).  d_preact is only read where activation is not 0.  No output may share memory with an
  * input or another output. */
 int skm_linear_backward(skm_ctx *ctx, int dtype, int activation, int64_t m, int64_t n, int64_t k, const void *d_dy,
                         int64_t lddy, const void *d_preact, int64_t ldp, const void *d_x, int64_t ldx, const void *d_w,

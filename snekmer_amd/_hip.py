@@ -303,8 +303,9 @@ def from_bfloat16(words) -> np.ndarray:
 class DeviceArray:
     """A typed 1-D/2-D view of device memory owned by a Context.  Other libraries read it in place through
     `__cuda_array_interface__` (torch.as_tensor(array, device="cuda"), cupy.asarray(array)); they have to order their own
-    streams behind the context's (Context.sync, or a context over their stream: Context(stream=...)).  bfloat16 has no
-    name there that every reader knows: pass such a library's own array as the output instead."""
+    streams behind the context's (Context.sync, or a context over their stream: Context(stream=...)), and the array has to live
+    until what they queued on a stream that no context knows has run: its memory is used again once the contexts' streams have
+    passed.  bfloat16 has no name there that every reader knows: pass such a library's own array as the output instead."""
 
     def __init__(self, ctx: "Context", shape, dtype):
         self.ctx = ctx
@@ -386,7 +387,11 @@ def _no() -> bool:
 def array_view(ctx: "Context", x, name: str, ndim: int, types, writable: bool = False):
     """(pointer, shape, row stride in elements, type string) of a device array of this library or of another one
     (`__cuda_array_interface__`), as the entry points take them: the elements of a row next to each other, rows that do not
-    overlap, on the context's device, of one of `types`.  Anything else raises TypeError / ValueError naming `name`."""
+    overlap, on the context's device, of one of `types`.  Anything else raises TypeError / ValueError naming `name`.
+
+    Nothing here waits.  The calls that take such arrays read and write them in the order of `ctx`'s stream: what another stream
+    (another context's, another library's) writes into them has to be finished first, or queued on a stream that the context
+    shares (Context(stream=...)), and their owner may let them go or write them again only behind the call."""
     if isinstance(x, DeviceArray):
         if x.ptr is None:
             raise ValueError(f"{name}: the array has been freed")

@@ -215,7 +215,8 @@ def log_probabilities(ctx, scores, labels=None, k: int = 0, temperature: float =
     may not be chosen either.  `temperature`: between 1e-30 and 1e30.  `k` <= 16 alternatives, padded with (-1, -inf).  A row that allows nothing has entropy 0 and
     log probability -inf; one that allows a NaN or +inf is NaN throughout, with indices -1.  A label on the device outside
     [-1, ncols) gives NaN and is reported by the next Context.sync / download.  `out`: a LogProbabilities whose members are
-    filled (arrays of this library or of another one); only those it has are computed."""
+    filled; only those it has are computed.  All arrays may be this library's or another one's (`_hip.array_view`: used in the
+    order of `ctx`'s stream, which their owners have to respect)."""
     args, keep = _score_arguments(ctx, scores, labels, mask, ncols, temperature)
     rows = args[1]
     k = int(k)
@@ -240,7 +241,8 @@ def log_probabilities_backward(ctx, scores, labels, forward: LogProbabilities, d
     """Gradient of ``(d_logp * logp + d_entropy * entropy).sum()`` with respect to the scores, in their type
     (skm_log_probabilities_backward).  `forward`: what `log_probabilities` left for the same scores, labels, mask and
     temperature (`stats`, and `entropy` if `d_entropy` is given).  Classes that may not be chosen get 0; columns of `out`
-    behind `ncols` are left as they are.  `out` may be `scores` itself.  Alternatives carry no gradient."""
+    behind `ncols` are left as they are.  `out` may be `scores` itself.  Alternatives carry no gradient.  Other libraries' arrays as in
+    `log_probabilities`."""
     args, keep = _score_arguments(ctx, scores, labels, mask, ncols, temperature)
     code, rows, cols = args[:3]
     if d_logp is None and d_entropy is None:

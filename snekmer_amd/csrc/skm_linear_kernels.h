@@ -60,8 +60,9 @@ struct ln_type<2> {
 };
 
 // ---- activations (in float32)
-// FINE: for float32 outputs, which keep that type's precision however small they are.  16-bit outputs are rounded at 2^-9 or
-// 2^-12 of themselves: the plain exponential, off by |x| u of itself (u = 2^-24: 6e-6 at x = -100), is exact enough for them.
+// FINE: for float32 outputs, which keep that type's precision however small they are (4096 x 4096 cells of k = 1024 with residual and
+// pre-activation: 272 us without activation, 274 with silu, 279 with gelu).  16-bit outputs are off by up to 2^-9 or 2^-12 of
+// themselves, by their rounding: the plain exponential, off by |x| u (u = 2^-24: 6e-6 at x = -100), is exact enough for them.
 
 // exp(x + x_lo) for x <= 0 (NaN stays) to 8 u: the rounding of x log2(e) is put back, and the square of exp(x / 2) reaches below
 // 2^-126, where the instruction's own results end
@@ -1055,7 +1056,7 @@ ln_plan plan_of(int dtype, int64_t cus, int64_t m, int64_t n, int64_t stages)
     return best;
 }
 
-// C = A B^T with the epilogue; a and b are ready (16-byte rows), CA / CB: across the contraction.
+// C = A B^T with the epilogue; a and b are as `ready` leaves them, CA / CB: across the contraction.
 template <int DT, bool CA = false, bool CB = false>
 int gemm(skm_ctx *ctx, ln_gemm g)
 {

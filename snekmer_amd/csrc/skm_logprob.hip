@@ -17,8 +17,8 @@
 // and the running list of the k best.  Rows with many tiles are shared by the waves of a workgroup, few long rows by
 // several workgroups whose partial states a second kernel joins.
 //
-// The k best of a tile: its lanes form G groups (G the power of two from k on), and no element below the k-th largest of the
-// group maxima can be among them, so only those above it (hardly more than k) are collected in LDS and ranked; equal ones
+// The k best of a tile: its lanes form G >= k groups (4, 8, 16, 32 for k up to 4, 8, 12, 16; the single lanes for k = 2), and no
+// element below the k-th largest of the group maxima can be among them, so only those above it (hardly more than k) are collected in LDS and ranked; equal ones
 // are taken in index order until k are held.  After the first tile only elements above the list's last one are looked at,
 // which costs one comparison a tile.
 //

@@ -603,8 +603,8 @@ def _expect(name: str, shape, want) -> None:
 
 def linear(ctx, x, w, bias=None, activation=None, residual=None, preact=None, out=None):
     """``act(x @ w.T + bias) + residual`` on the matrix cores (skm_linear): x [m, k], w [n, k], bias [n], residual [m, n], all
-    float32, float16 or `_hip.bfloat16`, arrays of this library or of another one (`_hip.array_view`; rows may be strided),
-    summed in float32.  `activation`: one of `ACTIVATIONS`.  `preact`: an array [m, n] that receives ``x @ w.T + bias``, or
+    float32, float16 or `_hip.bfloat16`, arrays of this library or of another one (`_hip.array_view`: used in the order of `ctx`'s stream, which their owners
+    have to respect; rows may be strided), summed in float32.  `activation`: one of `ACTIVATIONS`.  `preact`: an array [m, n] that receives ``x @ w.T + bias``, or
     True for a new one (the call then returns (y, preact)): what `linear_backward` needs for an activation.  `out` [m, n]: a new
     array unless given; it may be `residual` itself.  For feature rows under learned weights, where `cosine_dense_i8` compares
     count rows with each other."""
@@ -639,7 +639,10 @@ def linear(ctx, x, w, bias=None, activation=None, residual=None, preact=None, ou
 def linear_backward(ctx, dy, x, w, activation=None, preact=None, dx=True, dw=True, dbias=True):
     """The gradients of `linear` (skm_linear_backward): with ``dz = dy * act'(preact)``, ``dx = dz @ w``, ``dw = dz.T @ x`` and
     ``dbias = dz.sum(0)``; the residual's gradient is `dy` itself.  `dx`, `dw`, `dbias`: True for a new array, an array to fill,
-    or None / False where it is not wanted (`w` is only needed for dx, `x` only for dw; pass None).  Returns (dx, dw, dbias)."""
+    or None / False where it is not wanted (`w` is only needed for dx, `x` only for dw; pass None).  Returns (dx, dw, dbias).
+    With an activation, `dz` is rounded to the operands' type once before the two products, as mixed-precision training keeps it
+    (in 16 bits: dx and dw are off by 1.4 times what rounding them alone costs); `dbias` sums the unrounded values.  Other
+    libraries' arrays as in `linear`."""
     gp, gs, ldg, t = _hip.array_view(ctx, dy, "dy", 2, _hip.FLOAT_TYPES)
     types, code = (t,), _hip.FLOAT_TYPES[t]
     m, n = gs
