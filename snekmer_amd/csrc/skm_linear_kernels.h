@@ -61,7 +61,7 @@ struct ln_type<2> {
 
 // ---- activations (in float32)
 // FINE: for float32 outputs, which keep that type's precision however small they are (4096 x 4096 cells of k = 1024 with residual and
-// pre-activation: 272 us without activation, 274 with silu, 279 with gelu).  16-bit outputs are off by up to 2^-9 or 2^-12 of
+// pre-activation: 272 us without activation, 274 with silu, 279 with gelu).  16-bit outputs are off by up to 2^-8 or 2^-11 of
 // themselves, by their rounding: the plain exponential, off by |x| u (u = 2^-24: 6e-6 at x = -100), is exact enough for them.
 
 // exp(x + x_lo) for x <= 0 (NaN stays) to 8 u: the rounding of x log2(e) is put back, and the square of exp(x / 2) reaches below

@@ -172,6 +172,21 @@ def test_float32_activations_relative_to_themselves(ctx):
     assert (np.abs(y - want) <= (6 * np.abs(two_u) + 20) * U * np.abs(want) + tiny * np.abs(z)).all()
 
 
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("name, low", [("sigmoid", -80.0), ("silu", -80.0), ("gelu", -12.0), ("gelu_tanh", -9.0)])
+def test_activations_of_16_bits_relative_to_themselves(ctx, name, low, dt):
+    """The plain exponential is off by its argument's rounding, the argument times 2^-23 covers it (below 110: 2^-16), a dozen roundings of
+    float32 around it; half a step of the type follows."""
+    z, y, _ = one_term(ctx, np.linspace(low, 20.0, 1601), name, dt)
+    if name == "gelu":
+        want = z * 0.5 * np.vectorize(math.erfc)(-z / math.sqrt(2.0))
+    else:
+        u = 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3) if name == "gelu_tanh" else z
+        e = np.exp(-np.abs(u))
+        want = (1.0 if name == "sigmoid" else z) * np.where(u > 0, 1.0, e) / (1 + e)
+    assert (np.abs(y - want) <= (2.0 ** -15 + HALF_STEP[dt] * 1.01) * np.abs(want) + SMALLEST[dt]).all()
+
+
 @pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu", "sigmoid"])
 def test_float32_activations_keep_nan_and_reach_their_limits(ctx, name):
     z, y, slope = one_term(ctx, [np.nan, 300.0, -300.0, 2.0 ** 127, -2.0 ** 127, 0.0, -0.0], name, "f32")
