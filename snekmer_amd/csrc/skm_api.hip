@@ -340,18 +340,18 @@ int skm_check_device_error(skm_ctx *ctx, const char *who)
         "rows' log probabilities and gradients were set to NaN",
     };
     volatile uint32_t *w = (volatile uint32_t *)ctx->h_pinned + SKM_DEVERR_WORD;
-    std::string all;
+    char all[768] = "";
+    size_t len = 0;
     for (int i = 0; i < SKM_DEVERR_COUNT; ++i) {
         if (!w[i])
             continue;
         w[i] = 0;
-        if (!all.empty())
-            all += "; ";
-        all += TEXT[i];
+        if (len < sizeof(all))
+            len += (size_t)snprintf(all + len, sizeof(all) - len, "%s%s", len ? "; " : "", TEXT[i]);
     }
-    if (all.empty())
+    if (!len)
         return SKM_OK;
-    skm_set_error("%s: %s", who, all.c_str());
+    skm_set_error("%s: %s", who, all);
     return SKM_E_BADARG;
 }
 
